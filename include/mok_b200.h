@@ -496,6 +496,97 @@ int mokb_swiglu_bwd(const void* gate, const void* up, const void* d_hidden, void
                     const float* row_scale, float* row_grad_out, const int32_t* num_rows,
                     int64_t max_rows, int64_t cols, int has_limit, float limit, void* stream);
 
+/* ---- the layer for a few tokens (a decoding step).  No counterpart in the reference, whose layer takes 512 tokens or more.
+ *   y[t] = shared(x[t]) + sum_k router_weights[t, k] * expert_{top_experts[t, k]}(x[t])
+ * on one rank, without a schedule or a workspace of symmetric buffers.  The rank holds the experts [first_expert,
+ * first_expert + num_local_experts); routes to other experts, and routes whose weight is 0, contribute nothing and have
+ * nothing read for them, so with several ranks the sum of their results is the layer's (the shared expert on one of them).
+ * An expert may be named twice by a token.  A token without any result gets zeros.  In MXFP8 the routed experts multiply
+ * x and hidden quantised to E4M3 along the contraction (weights as in mokb_fwd_mxfp8_args); hidden is rounded to bf16 (or E4M3)
+ * between the products, everything else is fp32 until y is rounded.  Three launches; results do not depend on timing.
+ *   x, y [num_tokens, hidden] bf16, 16-byte aligned; top_experts [num_tokens, topk] int64; router_weights [num_tokens, topk]
+ *   hidden a multiple of 256, intermediate of 128; num_tokens in [0, MOKB_FEW_MAX_TOKENS]
+ *   workspace  mokb_few_tokens_workspace_bytes() bytes of the current device, 256-byte aligned, no initialisation needed, not
+ *              shared by calls that may overlap
+ *   the shared expert's three weights (bf16) may be NULL together */
+#define MOKB_FEW_MAX_TOKENS 511
+typedef struct {
+    int num_tokens, hidden, intermediate, num_local_experts, topk, first_expert;
+    int mxfp8;
+    int has_swiglu_limit;
+    float swiglu_limit;
+    const void* x;
+    const int64_t* top_experts;
+    const float* router_weights;
+    const void *w_shared_gate, *w_shared_up, *w_shared_down;      /* [I, H] [I, H] [H, I] */
+    const void *w_routed_gate, *w_routed_up, *w_routed_down;      /* [E_l, I, H] [E_l, I, H] [E_l, H, I], bf16 or E4M3 */
+    const void *w_routed_gate_sc, *w_routed_up_sc, *w_routed_down_sc;   /* MXFP8: packed scales */
+    void* y;
+    void* workspace;
+    int32_t* status;
+} mokb_few_tokens_args;
+size_t mokb_few_tokens_args_size(void);      /* sizeof(mokb_few_tokens_args) */
+size_t mokb_few_tokens_workspace_bytes(int num_tokens, int hidden, int intermediate, int topk, int mxfp8);   /* 0: bad sizes */
+int mokb_few_tokens_fwd(const mokb_few_tokens_args* args, void* stream);
+
+/* ---- the router (the reference takes its results ready made: tests/utils.py picks them with torch.topk).
+ * logits [num_tokens, num_experts] bf16 or fp32, rows `row_stride` elements apart -> top_experts [num_tokens, topk] int64 (what
+ * build_schedule takes), router_weights [num_tokens, topk].
+ *   MOKB_SCORE_SOFTMAX  s = softmax(logits), the largest logits are picked
+ *   MOKB_SCORE_SIGMOID  s = 1 / (1 + exp(-logits)), the largest s + bias are picked (bias [num_experts], optional; worked out in
+ *                       64 bits and compared as 32-bit numbers)
+ *   weights: scale * s of the picks, with `renormalize` divided by their sum
+ * Picks come in falling order, ties go to the lowest index; experts whose logit is -inf or NaN are closed: s = 0, picked only
+ * when nothing else is left, lowest index first, with weight 0.  +inf counts as the largest finite number.
+ * Load figures (optional, together; scratch: mokb_route_scratch_bytes()): tokens_per_expert [num_experts] int32, picks of open
+ * experts; score_sums [num_experts], the sum of s over the tokens in a fixed order.
+ * mokb_route_bwd: d_logits [num_tokens, num_experts] without gaps, in the logits' type, from d_router_weights and (optional)
+ * d_score_sums; top_experts are the forward call's (an entry outside [0, num_experts) is left out).  The picks themselves and
+ * tokens_per_expert have no gradient. */
+#define MOKB_SCORE_SOFTMAX 0
+#define MOKB_SCORE_SIGMOID 1
+#define MOKB_ROUTE_MAX_EXPERTS 1024
+#define MOKB_ROUTE_MAX_TOPK 32
+size_t mokb_route_scratch_bytes(int64_t num_tokens, int num_experts);
+int mokb_route(const void* logits, int bf16, int64_t row_stride, int64_t num_tokens, int num_experts, int topk, int score,
+               const float* bias, int renormalize, float scale, int64_t* top_experts, float* router_weights,
+               int32_t* tokens_per_expert, float* score_sums, void* scratch, void* stream);
+int mokb_route_bwd(const void* logits, int bf16, int64_t row_stride, int64_t num_tokens, int num_experts, int topk, int score,
+                   int renormalize, float scale, const int64_t* top_experts, const float* d_router_weights,
+                   const float* d_score_sums, void* d_logits, void* stream);
+
+/* ---- activations in 8 bits between forward and backward: [rows, cols] bf16 <-> q [rows, cols] int8 in [-127, 127] and scales
+ * [rows, ceil(cols / 128)] fp32, one per 128 values of a row (the last block of a row may be shorter); cols a multiple of 16.
+ * scale = max|x| / 127, q to the nearest, halves away from zero; blocks whose largest value is below 2^-110 are zeros, blocks
+ * with an infinity or NaN come back as NaN.  With num_rows (device, optional) only rows [0, min(*num_rows, rows)) are read and
+ * written, in all three.  Alignment: bf16 tensors 32 bytes, q 16.
+ * mokb_swiglu_bwd_packed: mokb_swiglu_bwd from packed gate and up, not rounded to bf16 in between; it also writes hidden
+ * [rows, cols].  Outputs must not overlap inputs. */
+int mokb_pack_rows(const void* x, void* q, float* scales, const int32_t* num_rows, int64_t rows, int64_t cols, void* stream);
+int mokb_unpack_rows(const void* q, const float* scales, void* x, const int32_t* num_rows, int64_t rows, int64_t cols, void* stream);
+int mokb_swiglu_bwd_packed(const void* gate_q, const float* gate_scales, const void* up_q, const float* up_scales,
+                           const void* d_hidden, void* d_gate, void* d_up, void* hidden, const float* row_scale,
+                           float* row_grad_out, const int32_t* num_rows, int64_t rows, int64_t cols, int has_limit, float limit,
+                           void* stream);
+
+/* The BF16 backward pass from a context in that form: x_routed, gate and up of the routed rows (macrobatch 0) and gate and up
+ * of the shared expert.  Of mokb_bwd_bf16_args, x_routed [MB, H], hidden_routed [MB, I] and hidden_shared [T, I] are then work
+ * buffers without contents, and so are gate_routed and up_routed [MB, I], which are needed only when schedule_capacity >
+ * macrobatch_size (the replay of later macrobatches) and may be NULL otherwise; gate_shared and up_shared are not used. */
+typedef struct {
+    const void* x_routed_q;
+    const float* x_routed_scales;
+    const void* gate_routed_q;
+    const float* gate_routed_scales;
+    const void* up_routed_q;
+    const float* up_routed_scales;
+    const void* gate_shared_q;
+    const float* gate_shared_scales;
+    const void* up_shared_q;
+    const float* up_shared_scales;
+} mokb_packed_context;
+int mokb_dispatch_mlp_swiglu_combine_bwd_bf16_packed(const mokb_bwd_bf16_args* args, const mokb_packed_context* context, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

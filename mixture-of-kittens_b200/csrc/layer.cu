@@ -178,14 +178,22 @@ extern "C" int mokb_dispatch_mlp_swiglu_combine_fwd_bf16(const mokb_fwd_bf16_arg
     return MOKB_OK;
 }
 
-extern "C" int mokb_dispatch_mlp_swiglu_combine_bwd_bf16(const mokb_bwd_bf16_args* a, void* stream_) {
-    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+// `packed`: the saved context in 8 bits (pack.cu); the context pointers of `a` are then work buffers.
+static int backward_bf16(const mokb_bwd_bf16_args* a, const mokb_packed_context* packed, cudaStream_t stream) {
     MOKB_TRY(check_common(a, "bwd_bf16"));
     MOKB_REQUIRE(a->d_y_ptrs_host && a->d_x_routed_ptrs_host && a->router_weight_ptrs_host && a->d_router_weight_ptrs_host && a->x_ptrs_host,
                  "bwd_bf16: null pointer list");
     MOKB_REQUIRE(a->w_shared_gate && a->w_shared_up && a->w_shared_down && a->w_routed_gate && a->w_routed_up && a->w_routed_down, "bwd_bf16: null weight");
-    MOKB_REQUIRE(a->x_routed && a->gate_shared && a->gate_routed && a->up_shared && a->up_routed && a->hidden_shared && a->hidden_routed,
-                 "bwd_bf16: null forward context");
+    if (packed) {
+        MOKB_REQUIRE(packed->x_routed_q && packed->x_routed_scales && packed->gate_routed_q && packed->gate_routed_scales && packed->up_routed_q &&
+                     packed->up_routed_scales && packed->gate_shared_q && packed->gate_shared_scales && packed->up_shared_q && packed->up_shared_scales,
+                     "bwd_bf16: null packed context");
+        MOKB_REQUIRE(a->x_routed && a->hidden_shared && a->hidden_routed, "bwd_bf16: null work buffer");
+        MOKB_REQUIRE(a->schedule_capacity <= a->macrobatch_size || (a->gate_routed && a->up_routed), "bwd_bf16: the replay needs gate_routed and up_routed");
+    } else {
+        MOKB_REQUIRE(a->x_routed && a->gate_shared && a->gate_routed && a->up_shared && a->up_routed && a->hidden_shared && a->hidden_routed,
+                     "bwd_bf16: null forward context");
+    }
     MOKB_REQUIRE(a->d_x_shared && a->d_gate_shared && a->d_gate_routed && a->d_up_shared && a->d_up_routed &&
                  a->d_hidden_shared && a->d_hidden_routed && a->d_y_routed && a->d_w_shared_gate && a->d_w_routed_gate &&
                  a->d_w_shared_up && a->d_w_routed_up && a->d_w_shared_down && a->d_w_routed_down, "bwd_bf16: null output");
@@ -244,8 +252,13 @@ extern "C" int mokb_dispatch_mlp_swiglu_combine_bwd_bf16(const mokb_bwd_bf16_arg
             g.mode = 2; g.rows_static = T; g.N = I; g.K = H;
             g.A = d_y_local; g.lda = H; g.B = a->w_shared_down; g.ldb = I; g.D = a->d_hidden_shared; g.ldd = I;
             MOKB_TRY(mokb_grouped_gemm_bf16(&g, stream));
-            MOKB_TRY(mokb_swiglu_bwd(a->gate_shared, a->up_shared, a->d_hidden_shared, a->d_gate_shared, a->d_up_shared, nullptr, nullptr,
-                                     nullptr, T, I, lim, limv, stream));
+            if (packed)
+                MOKB_TRY(mokb_swiglu_bwd_packed(packed->gate_shared_q, packed->gate_shared_scales, packed->up_shared_q, packed->up_shared_scales,
+                                                a->d_hidden_shared, a->d_gate_shared, a->d_up_shared, const_cast<void*>(a->hidden_shared), nullptr,
+                                                nullptr, nullptr, T, I, lim, limv, stream));
+            else
+                MOKB_TRY(mokb_swiglu_bwd(a->gate_shared, a->up_shared, a->d_hidden_shared, a->d_gate_shared, a->d_up_shared, nullptr, nullptr,
+                                         nullptr, T, I, lim, limv, stream));
             g = gemm_base(a->status);
             g.mode = 2; g.rows_static = T; g.N = H; g.K = I;
             g.A = a->d_gate_shared; g.B = a->w_shared_gate; g.A2 = a->d_up_shared; g.B2 = a->w_shared_up; g.lda = I; g.ldb = H;
@@ -277,8 +290,15 @@ extern "C" int mokb_dispatch_mlp_swiglu_combine_bwd_bf16(const mokb_bwd_bf16_arg
         MOKB_TRY(mokb_grouped_gemm_bf16(&g, stream));
         // (the pulls have all arrived once that GEMM is through its last window; the event makes it formal)
         if (flags) MOKB_CUDA(cudaStreamWaitEvent(stream, as->join2, 0));
-        MOKB_TRY(mokb_swiglu_bwd(a->gate_routed, a->up_routed, a->d_hidden_routed, a->d_gate_routed, a->d_up_routed, s.w_row, s.d_w_row,
-                                 s.mb_rows + m, MB, I, lim, limv, stream));
+        if (packed && m == 0) {
+            MOKB_TRY(mokb_swiglu_bwd_packed(packed->gate_routed_q, packed->gate_routed_scales, packed->up_routed_q, packed->up_routed_scales,
+                                            a->d_hidden_routed, a->d_gate_routed, a->d_up_routed, const_cast<void*>(a->hidden_routed), s.w_row,
+                                            s.d_w_row, s.mb_rows, MB, I, lim, limv, stream));
+            MOKB_TRY(mokb_unpack_rows(packed->x_routed_q, packed->x_routed_scales, const_cast<void*>(a->x_routed), s.mb_rows, MB, H, stream));
+        } else {
+            MOKB_TRY(mokb_swiglu_bwd(a->gate_routed, a->up_routed, a->d_hidden_routed, a->d_gate_routed, a->d_up_routed, s.w_row, s.d_w_row,
+                                     s.mb_rows + m, MB, I, lim, limv, stream));
+        }
         // d_x = d_gate * W_gate + d_up * W_up; the epilogue stores every row straight into slot t*K+k of its home rank's
         // d_x_routed buffer, and the route's router-weight gradient with it (the reverse dispatch)
         g = gemm_base(a->status);
@@ -297,4 +317,13 @@ extern "C" int mokb_dispatch_mlp_swiglu_combine_bwd_bf16(const mokb_bwd_bf16_arg
                                   a->d_w_routed_gate, a->d_w_routed_up, H, I, E_l, lo, hi - lo, offs, k_end, m > 0, a->status, stream));
     }
     return MOKB_OK;
+}
+
+extern "C" int mokb_dispatch_mlp_swiglu_combine_bwd_bf16(const mokb_bwd_bf16_args* a, void* stream) {
+    return backward_bf16(a, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int mokb_dispatch_mlp_swiglu_combine_bwd_bf16_packed(const mokb_bwd_bf16_args* a, const mokb_packed_context* context, void* stream) {
+    MOKB_REQUIRE(context != nullptr, "bwd_bf16: null packed context");
+    return backward_bf16(a, context, static_cast<cudaStream_t>(stream));
 }

@@ -1,0 +1,234 @@
+// Activations kept in 8 bits between the forward and the backward pass: whole numbers in [-127, 127] with one fp32 scale per 128
+// consecutive values of a row, 1.03 bytes a value instead of 2.
+//
+//   scale = max|x| / 127,  q = x / scale to the nearest, halves away from zero;   x ~ q * scale, off by at most half a step
+// Of values drawn from one distribution that is three to four times nearer than E4M3 with a scale per 32 (whose step grows with the
+// value), which is why this is not the layer's MXFP8 form.  A block whose largest value is below 2^-110 is kept as zeros; one that holds
+// an infinity or NaN comes back as NaN, so that a fault stays visible.
+//
+//   pack_kernel        bf16 -> q, scales
+//   unpack_kernel      q, scales -> bf16 (the x rows, which a weight-gradient GEMM reads)
+//   swiglu_bwd_packed  the backward pass of SwiGLU straight from packed gate and up; gives `hidden` back as well, so the
+//                      forward pass keeps two of its three [rows, I] tensors, in half the bytes
+// All bound by HBM.  A lane works on 16 consecutive values: 32 bytes of bf16, 16 of q; eight lanes have one scale.
+#include "common.cuh"
+#include "mxfp8_codec.cuh"
+
+namespace mokb {
+namespace {
+
+constexpr int kBlock = 128;
+constexpr float kSmallest = 7.70371977754894e-34f;        // 2^-110
+
+__device__ __forceinline__ int64_t live_rows(const int32_t* num_rows, int64_t cap) {
+    if (!num_rows) return cap;
+    const int64_t n = *num_rows;
+    return n < 0 ? 0 : n < cap ? n : cap;
+}
+
+// 16-byte loads and stores of bytes that are used once
+__device__ __forceinline__ uint4 ld_once(const void* p) { return __ldcs(static_cast<const uint4*>(p)); }
+
+// Eight lanes hold a block's 128 values (16 each, as bf16 pairs): q as bytes, and the scale, the same in all eight.
+__device__ __forceinline__ uint4 pack_16(const uint32_t (&w)[8], float* scale) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);           // of the bits: NaN above infinity above numbers
+    m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float top = __uint_as_float(m << 16);
+    const bool bad = m >= 0x7f80u;
+    *scale = bad ? __int_as_float(0x7fffffff) : top >= kSmallest ? __fdiv_rn(top, 127.0f) : 0.0f;
+    // 127 / top, a little (2^-18) more: with 8-bit fractions x * 127 / top is a half exactly or at least 1.5e-5 of itself away from one,
+    // so halves go away from zero and nothing else moves
+    const float inv = bad || top < kSmallest ? 0.0f : __fdiv_rn(127.0f * (1.0f + 3.814697265625e-6f), top);
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t word = 0u;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t pair = w[2 * i + j];
+            const int a = bad ? 0 : __float2int_rn(bf16_lo(pair) * inv), b = bad ? 0 : __float2int_rn(bf16_hi(pair) * inv);
+            word |= ((static_cast<uint32_t>(a) & 0xffu) | (static_cast<uint32_t>(b) & 0xffu) << 8) << (16 * j);
+        }
+        o[i] = word;
+    }
+    return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// byte j of a word as a signed number
+__device__ __forceinline__ float signed_byte(uint32_t w, int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); }
+
+// A warp takes four blocks at a time.  `per_row` blocks of a row, the last one shorter where 128 does not divide cols.
+__global__ void __launch_bounds__(256) pack_kernel(const __nv_bfloat16* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scales,
+                                                   const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row) {
+    const int64_t items = live_rows(num_rows, rows_cap) * per_row * 8, stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    const int lane = threadIdx.x & 31;
+    const bool even = cols % kBlock == 0;
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x - lane; i0 < items; i0 += stride) {      // the same trips in a warp
+        const int64_t i = i0 + lane, block = i >> 3;
+        int64_t at = i * 16;
+        bool inside = i < items;
+        if (!even) {
+            const int64_t row = block / per_row;
+            const int c = static_cast<int>(block - row * per_row) * kBlock + static_cast<int>(i & 7) * 16;
+            inside = inside && c < cols;
+            at = row * cols + c;
+        }
+        uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+        if (inside) ld_global_32B(x + at, w);
+        float scale;
+        const uint4 o = pack_16(w, &scale);
+        if (inside) *reinterpret_cast<uint4*>(q + at) = o;
+        if ((i & 7) == 0 && i < items) scales[block] = scale;
+    }
+}
+
+__global__ void __launch_bounds__(256) unpack_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales, __nv_bfloat16* __restrict__ x,
+                                                     const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row) {
+    const int64_t items = live_rows(num_rows, rows_cap) * (cols / 16), stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    const int units = cols / 16;
+    const bool even = cols % kBlock == 0;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += stride) {
+        int64_t block = i >> 3;
+        if (!even) {
+            const int64_t row = i / units;
+            block = row * per_row + (i - row * units) / 8;
+        }
+        const uint4 v = ld_once(q + i * 16);
+        const float s = __ldg(scales + block);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            o[2 * j] = pack2(signed_byte(w[j], 0) * s, signed_byte(w[j], 1) * s);
+            o[2 * j + 1] = pack2(signed_byte(w[j], 2) * s, signed_byte(w[j], 3) * s);
+        }
+        st_global_32B(x + i * 16, o);
+    }
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
+
+// One warp per row; the row's sum of d_hidden * hidden, divided by its router weight, in a fixed order.
+__global__ void __launch_bounds__(256) swiglu_bwd_packed_kernel(
+    const int8_t* __restrict__ gate_q, const float* __restrict__ gate_sc, const int8_t* __restrict__ up_q, const float* __restrict__ up_sc,
+    const __nv_bfloat16* __restrict__ d_hidden, __nv_bfloat16* __restrict__ d_gate, __nv_bfloat16* __restrict__ d_up,
+    __nv_bfloat16* __restrict__ hidden, const float* __restrict__ row_scale, float* __restrict__ row_grad,
+    const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row, int has_limit, float limit) {
+    const int64_t rows = live_rows(num_rows, rows_cap), warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
+    const int lane = threadIdx.x & 31, units = cols / 16;
+    const float lim = has_limit ? limit : __int_as_float(0x7f800000);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); row < rows; row += warps) {
+        float sum = 0.0f;
+        float inv_w = 1.0f;
+        if (row_grad && row_scale) {
+            const float w = row_scale[row];
+            inv_w = w > 0.0f ? 1.0f / w : 0.0f;
+        }
+        for (int u = lane; u < units; u += 32) {
+            const int64_t at = row * cols + u * 16, block = row * per_row + (u >> 3);
+            const uint4 gv = ld_once(gate_q + at), uv = ld_once(up_q + at);
+            uint32_t dh[8];
+            ld_global_32B(d_hidden + at, dh);
+            const float gs = __ldg(gate_sc + block), us = __ldg(up_sc + block);
+            const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+            uint32_t og[8], ou[8], oh[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float dg[2], du[2], h[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const int byte = 2 * (j & 1) + b;
+                    const float g0 = signed_byte(gw[j >> 1], byte) * gs, u0 = signed_byte(uw[j >> 1], byte) * us;
+                    const float d = b ? bf16_hi(dh[j]) : bf16_lo(dh[j]);
+                    const float g = min_nan(g0, lim), up = min_nan(max_nan(u0, -lim), lim);
+                    const float sig = 1.0f / (1.0f + __expf(-g));          // (IEEE: the approximate quotient is zero for gates near -88)
+                    const float silu = g * sig;
+                    h[b] = silu * up;
+                    dg[b] = g0 > lim ? 0.0f : ((1.0f - silu) * sig + silu) * up * d;
+                    du[b] = u0 > lim || u0 < -lim ? 0.0f : silu * d;
+                    sum += d * inv_w * h[b];
+                }
+                og[j] = pack2(dg[0], dg[1]);
+                ou[j] = pack2(du[0], du[1]);
+                oh[j] = pack2(h[0], h[1]);
+            }
+            st_global_32B(d_gate + at, og);
+            st_global_32B(d_up + at, ou);
+            st_global_32B(hidden + at, oh);
+        }
+        if (row_grad) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane == 0) row_grad[row] = sum;
+        }
+    }
+}
+
+int blocks_for(int64_t threads, int per_sm) {
+    int64_t b = (threads + 255) / 256;
+    const int64_t most = static_cast<int64_t>(sm_count()) * per_sm;
+    if (b > most) b = most;
+    return b < 1 ? 1 : static_cast<int>(b);
+}
+
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+}  // namespace
+}  // namespace mokb
+
+using namespace mokb;
+
+#define CHECK_PACK(who)                                                                                                              \
+    MOKB_REQUIRE(rows >= 0 && cols > 0 && cols % 16 == 0 && cols <= (1 << 24), who ": cols must be a positive multiple of 16")
+
+extern "C" int mokb_pack_rows(const void* x, void* q, float* scales, const int32_t* num_rows, int64_t rows, int64_t cols, void* stream) {
+    TraceScope trace(static_cast<cudaStream_t>(stream), "pack_rows");
+    CHECK_PACK("pack_rows");
+    if (rows == 0) return MOKB_OK;
+    MOKB_REQUIRE(x && q && scales, "pack_rows: null pointer");
+    MOKB_REQUIRE(aligned(x, 32) && aligned(q, 16), "pack_rows: x must be 32-byte and q 16-byte aligned");
+    const int per_row = static_cast<int>((cols + kBlock - 1) / kBlock);
+    pack_kernel<<<blocks_for(rows * per_row * 8, 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const __nv_bfloat16*>(x), static_cast<int8_t*>(q), scales, num_rows, rows, static_cast<int>(cols), per_row);
+    MOKB_CUDA(cudaGetLastError());
+    note_launch();
+    return MOKB_OK;
+}
+
+extern "C" int mokb_unpack_rows(const void* q, const float* scales, void* x, const int32_t* num_rows, int64_t rows, int64_t cols, void* stream) {
+    TraceScope trace(static_cast<cudaStream_t>(stream), "unpack_rows");
+    CHECK_PACK("unpack_rows");
+    if (rows == 0) return MOKB_OK;
+    MOKB_REQUIRE(x && q && scales, "unpack_rows: null pointer");
+    MOKB_REQUIRE(aligned(x, 32) && aligned(q, 16), "unpack_rows: x must be 32-byte and q 16-byte aligned");
+    unpack_kernel<<<blocks_for(rows * (cols / 16), 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const int8_t*>(q), scales, static_cast<__nv_bfloat16*>(x), num_rows, rows, static_cast<int>(cols),
+        static_cast<int>((cols + kBlock - 1) / kBlock));
+    MOKB_CUDA(cudaGetLastError());
+    note_launch();
+    return MOKB_OK;
+}
+
+extern "C" int mokb_swiglu_bwd_packed(const void* gate_q, const float* gate_scales, const void* up_q, const float* up_scales,
+                                      const void* d_hidden, void* d_gate, void* d_up, void* hidden, const float* row_scale,
+                                      float* row_grad_out, const int32_t* num_rows, int64_t rows, int64_t cols, int has_limit, float limit,
+                                      void* stream) {
+    TraceScope trace(static_cast<cudaStream_t>(stream), "swiglu_bwd_packed");
+    CHECK_PACK("swiglu_bwd_packed");
+    if (rows == 0) return MOKB_OK;
+    MOKB_REQUIRE(gate_q && gate_scales && up_q && up_scales && d_hidden && d_gate && d_up && hidden, "swiglu_bwd_packed: null pointer");
+    MOKB_REQUIRE(aligned(gate_q, 16) && aligned(up_q, 16) && aligned(d_hidden, 32) && aligned(d_gate, 32) && aligned(d_up, 32) && aligned(hidden, 32),
+                 "swiglu_bwd_packed: packed tensors must be 16-byte and bf16 tensors 32-byte aligned");
+    swiglu_bwd_packed_kernel<<<blocks_for(rows * 32, 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const int8_t*>(gate_q), gate_scales, static_cast<const int8_t*>(up_q), up_scales, static_cast<const __nv_bfloat16*>(d_hidden),
+        static_cast<__nv_bfloat16*>(d_gate), static_cast<__nv_bfloat16*>(d_up), static_cast<__nv_bfloat16*>(hidden), row_scale, row_grad_out,
+        num_rows, rows, static_cast<int>(cols), static_cast<int>((cols + kBlock - 1) / kBlock), has_limit, limit);
+    MOKB_CUDA(cudaGetLastError());
+    note_launch();
+    return MOKB_OK;
+}

@@ -95,6 +95,21 @@ class GemmFp8Args(ctypes.Structure):
            ("reserve_sms", c_int), ("group_k_end", c_vp), ("D3", c_vp)])
 
 
+class FewTokensArgs(ctypes.Structure):
+    _fields_ = (
+        [(n, c_int) for n in ("num_tokens", "hidden", "intermediate", "num_local_experts", "topk", "first_expert", "mxfp8",
+                              "has_swiglu_limit")]
+        + [("swiglu_limit", c_f32)]
+        + [(n, c_vp) for n in ("x", "top_experts", "router_weights", "w_shared_gate", "w_shared_up", "w_shared_down",
+                               "w_routed_gate", "w_routed_up", "w_routed_down", "w_routed_gate_sc", "w_routed_up_sc",
+                               "w_routed_down_sc", "y", "workspace", "status")])
+
+
+class PackedContext(ctypes.Structure):
+    _fields_ = [(f"{n}_{part}", c_vp) for n in ("x_routed", "gate_routed", "up_routed", "gate_shared", "up_shared")
+                for part in ("q", "scales")]
+
+
 def _sig(name, restype, *argtypes):
     fn = getattr(lib, name)
     fn.restype = restype
@@ -134,6 +149,16 @@ _sig("mokb_combine_rows_window", c_int, c_vp, c_u64p, c_int, c_vp, c_vp, c_vp, c
      c_int, c_vp, c_i64, c_vp)
 _sig("mokb_swiglu_fwd", c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_f32, c_vp)
 _sig("mokb_swiglu_bwd", c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_f32, c_vp)
+_sig("mokb_few_tokens_args_size", c_sz)
+_sig("mokb_few_tokens_workspace_bytes", c_sz, c_int, c_int, c_int, c_int, c_int)
+_sig("mokb_few_tokens_fwd", c_int, ctypes.POINTER(FewTokensArgs), c_vp)
+_sig("mokb_route_scratch_bytes", c_sz, c_i64, c_int)
+_sig("mokb_route", c_int, c_vp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_vp, c_int, c_f32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp)
+_sig("mokb_route_bwd", c_int, c_vp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_int, c_f32, c_vp, c_vp, c_vp, c_vp, c_vp)
+_sig("mokb_pack_rows", c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp)
+_sig("mokb_unpack_rows", c_int, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_vp)
+_sig("mokb_swiglu_bwd_packed", c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_int, c_f32, c_vp)
+_sig("mokb_dispatch_mlp_swiglu_combine_bwd_bf16_packed", c_int, ctypes.POINTER(BwdArgs), ctypes.POINTER(PackedContext), c_vp)
 
 EXPORTED = [
     "mokb_last_error", "mokb_device_arch", "mokb_sm_count", "mokb_struct_sizes", "mokb_set_barrier_timeout_ms", "mokb_launch_count",
@@ -143,6 +168,9 @@ EXPORTED = [
     "mokb_dispatch_mlp_swiglu_combine_fwd_bf16", "mokb_dispatch_mlp_swiglu_combine_bwd_bf16",
     "mokb_grouped_gemm_bf16", "mokb_grouped_gemm_mxfp8", "mokb_dispatch_rows", "mokb_combine_rows", "mokb_swiglu_fwd", "mokb_swiglu_bwd",
     "mokb_comm_default_blocks", "mokb_dispatch_rows_window", "mokb_dispatch_rows_quant", "mokb_combine_rows_window",
+    "mokb_few_tokens_args_size", "mokb_few_tokens_workspace_bytes", "mokb_few_tokens_fwd",
+    "mokb_route_scratch_bytes", "mokb_route", "mokb_route_bwd",
+    "mokb_pack_rows", "mokb_unpack_rows", "mokb_swiglu_bwd_packed", "mokb_dispatch_mlp_swiglu_combine_bwd_bf16_packed",
 ]
 
 
@@ -171,6 +199,8 @@ def _check_struct_layout():
     mine = (ctypes.sizeof(FwdArgs), ctypes.sizeof(BwdArgs), ctypes.sizeof(GemmArgs))
     if tuple(sizes) != mine:
         raise ImportError(f"struct layout mismatch between _C.py {mine} and libmok_b200.so {tuple(sizes)}")
+    if ctypes.sizeof(FewTokensArgs) != lib.mokb_few_tokens_args_size():
+        raise ImportError("struct layout mismatch between _C.py and libmok_b200.so: FewTokensArgs")
 
 
 _check_struct_layout()
@@ -431,13 +461,13 @@ def recompute_forward_context_bf16(x, x_ptrs, w_shared_gate, w_routed_gate, w_sh
                      num_comm_sms, macrobatch_size, minibatch_size, True)[:7]
 
 
-def dispatch_mlp_swiglu_combine_bwd_bf16(d_y_buffer, d_y_buffer_ptrs, d_x_routed_buffer, d_x_routed_buffer_ptrs,
-                                         router_weight_buffer, router_weight_buffer_ptrs, d_router_weight_buffer,
-                                         d_router_weight_buffer_ptrs, w_shared_gate, w_routed_gate, w_shared_up,
-                                         w_routed_up, w_shared_down, w_routed_down, x_routed, gate_shared, gate_routed,
-                                         up_shared, up_routed, hidden_shared, hidden_routed, x, x_ptrs,
-                                         schedule_peer_rank, schedule_peer_token_idx, num_tokens, tokens_per_expert,
-                                         topk, swiglu_limit, num_comm_sms, macrobatch_size, minibatch_size):
+def _bwd_bf16(d_y_buffer, d_y_buffer_ptrs, d_x_routed_buffer, d_x_routed_buffer_ptrs,
+              router_weight_buffer, router_weight_buffer_ptrs, d_router_weight_buffer,
+              d_router_weight_buffer_ptrs, w_shared_gate, w_routed_gate, w_shared_up,
+              w_routed_up, w_shared_down, w_routed_down, x_routed, gate_shared, gate_routed,
+              up_shared, up_routed, hidden_shared, hidden_routed, x, x_ptrs,
+              schedule_peer_rank, schedule_peer_token_idx, num_tokens, tokens_per_expert,
+              topk, swiglu_limit, num_comm_sms, macrobatch_size, minibatch_size, packed=None):
     a = BwdArgs()
     T, H, I, E_l, dev, scratch = _common(
         a, x_ptrs=x_ptrs, x_like=x, w_shared_gate=w_shared_gate, w_routed_gate=w_routed_gate,
@@ -471,10 +501,130 @@ def dispatch_mlp_swiglu_combine_bwd_bf16(d_y_buffer, d_y_buffer_ptrs, d_x_routed
     a.d_w_shared_gate, a.d_w_routed_gate, a.d_w_shared_up, a.d_w_routed_up = (_p(d_w_shared_gate), _p(d_w_routed_gate),
                                                                              _p(d_w_shared_up), _p(d_w_routed_up))
     a.d_w_shared_down, a.d_w_routed_down = _p(d_w_shared_down), _p(d_w_routed_down)
-    _ck(lib.mokb_dispatch_mlp_swiglu_combine_bwd_bf16(ctypes.byref(a), _stream()))
+    if packed is None:
+        _ck(lib.mokb_dispatch_mlp_swiglu_combine_bwd_bf16(ctypes.byref(a), _stream()))
+    else:
+        c = PackedContext(*[_p(t) for t in packed])
+        _ck(lib.mokb_dispatch_mlp_swiglu_combine_bwd_bf16_packed(ctypes.byref(a), ctypes.byref(c), _stream()))
     return (d_x_shared, d_x_routed, d_gate_shared, d_gate_routed, d_up_shared, d_up_routed, d_hidden_shared,
             d_hidden_routed, d_y_routed, d_w_shared_gate, d_w_routed_gate, d_w_shared_up, d_w_routed_up,
             d_w_shared_down, d_w_routed_down)
+
+
+def dispatch_mlp_swiglu_combine_bwd_bf16(d_y_buffer, d_y_buffer_ptrs, d_x_routed_buffer, d_x_routed_buffer_ptrs,
+                                         router_weight_buffer, router_weight_buffer_ptrs, d_router_weight_buffer,
+                                         d_router_weight_buffer_ptrs, w_shared_gate, w_routed_gate, w_shared_up,
+                                         w_routed_up, w_shared_down, w_routed_down, x_routed, gate_shared, gate_routed,
+                                         up_shared, up_routed, hidden_shared, hidden_routed, x, x_ptrs,
+                                         schedule_peer_rank, schedule_peer_token_idx, num_tokens, tokens_per_expert,
+                                         topk, swiglu_limit, num_comm_sms, macrobatch_size, minibatch_size):
+    return _bwd_bf16(d_y_buffer, d_y_buffer_ptrs, d_x_routed_buffer, d_x_routed_buffer_ptrs, router_weight_buffer,
+                     router_weight_buffer_ptrs, d_router_weight_buffer, d_router_weight_buffer_ptrs, w_shared_gate,
+                     w_routed_gate, w_shared_up, w_routed_up, w_shared_down, w_routed_down, x_routed, gate_shared,
+                     gate_routed, up_shared, up_routed, hidden_shared, hidden_routed, x, x_ptrs, schedule_peer_rank,
+                     schedule_peer_token_idx, num_tokens, tokens_per_expert, topk, swiglu_limit, num_comm_sms,
+                     macrobatch_size, minibatch_size)
+
+
+def dispatch_mlp_swiglu_combine_bwd_bf16_packed(d_y_buffer, d_y_buffer_ptrs, d_x_routed_buffer, d_x_routed_buffer_ptrs,
+                                                router_weight_buffer, router_weight_buffer_ptrs, d_router_weight_buffer,
+                                                d_router_weight_buffer_ptrs, w_shared_gate, w_routed_gate, w_shared_up,
+                                                w_routed_up, w_shared_down, w_routed_down, packed, x, x_ptrs,
+                                                schedule_peer_rank, schedule_peer_token_idx, num_tokens,
+                                                tokens_per_expert, topk, swiglu_limit, num_comm_sms, macrobatch_size,
+                                                minibatch_size):
+    """`packed`: q and scales of x_routed, gate_routed, up_routed, gate_shared, up_shared.  What the kernels rebuild of the
+    context lives only as long as the call."""
+    T, H = x.shape
+    I = w_shared_gate.shape[0]
+    MB = macrobatch_size
+    bf = dict(dtype=torch.bfloat16, device=x.device)
+    replay = schedule_peer_rank.numel() > MB
+    gate_routed, up_routed = (torch.empty(MB, I, **bf) if replay else None for _ in range(2))
+    return _bwd_bf16(d_y_buffer, d_y_buffer_ptrs, d_x_routed_buffer, d_x_routed_buffer_ptrs, router_weight_buffer,
+                     router_weight_buffer_ptrs, d_router_weight_buffer, d_router_weight_buffer_ptrs, w_shared_gate,
+                     w_routed_gate, w_shared_up, w_routed_up, w_shared_down, w_routed_down, torch.empty(MB, H, **bf),
+                     None, gate_routed, None, up_routed, torch.empty(T, I, **bf), torch.empty(MB, I, **bf), x, x_ptrs,
+                     schedule_peer_rank, schedule_peer_token_idx, num_tokens, tokens_per_expert, topk, swiglu_limit,
+                     num_comm_sms, macrobatch_size, minibatch_size, packed)
+
+
+# ----------------------------------------------------------------------------
+# Operators around the layer: router, few tokens, activations in 8 bits
+# ----------------------------------------------------------------------------
+PACK_BLOCK = 128
+
+
+def route(logits, bias, topk, sigmoid, renormalize, scale, balance):
+    T, E = logits.shape
+    dev = logits.device
+    top_experts = torch.empty(T, topk, dtype=torch.int64, device=dev)
+    weights = torch.empty(T, topk, dtype=torch.float32, device=dev)
+    counts = sums = scratch = None
+    if balance:
+        counts = torch.empty(E, dtype=torch.int32, device=dev)
+        sums = torch.empty(E, dtype=torch.float32, device=dev)
+        scratch = torch.empty(lib.mokb_route_scratch_bytes(T, E), dtype=torch.uint8, device=dev)
+    _ck(lib.mokb_route(_p(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if T > 1 else E, T, E, topk, int(sigmoid),
+                       _p(bias), int(renormalize), scale, _p(top_experts), _p(weights), _p(counts), _p(sums), _p(scratch),
+                       _stream()))
+    return top_experts, weights, counts, sums
+
+
+def route_bwd(logits, top_experts, d_router_weights, d_score_sums, sigmoid, renormalize, scale):
+    T, E = logits.shape
+    d_logits = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
+    _ck(lib.mokb_route_bwd(_p(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if T > 1 else E, T, E,
+                           top_experts.shape[1], int(sigmoid), int(renormalize), scale, _p(top_experts), _p(d_router_weights),
+                           _p(d_score_sums), _p(d_logits), _stream()))
+    return d_logits
+
+
+def few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w_shared_down, w_routed_gate, w_routed_up,
+                   w_routed_down, scales, first_expert, swiglu_limit):
+    """`scales`: None, or the packed scales of the three routed weights (MXFP8).  The work area is a tensor of this call:
+    calls on several streams, or captured in several graphs, do not share it."""
+    T, H = x.shape
+    E, I = w_routed_gate.shape[:2]
+    K = top_experts.shape[1]
+    mx = int(scales is not None)
+    y = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
+    work = torch.empty(lib.mokb_few_tokens_workspace_bytes(T, H, I, K, mx), dtype=torch.uint8, device=x.device)
+    a = FewTokensArgs(T, H, I, E, K, first_expert, mx, 0 if swiglu_limit is None else 1,
+                      0.0 if swiglu_limit is None else float(swiglu_limit), _p(x), _p(top_experts), _p(router_weights),
+                      _p(w_shared_gate), _p(w_shared_up), _p(w_shared_down), _p(w_routed_gate), _p(w_routed_up),
+                      _p(w_routed_down), *((None,) * 3 if scales is None else map(_p, scales)), _p(y), _p(work),
+                      _p(status_tensor(x.device)))
+    _ck(lib.mokb_few_tokens_fwd(ctypes.byref(a), _stream()))
+    return y
+
+
+def _packed_like(x):
+    rows, cols = x.shape
+    return (torch.empty(rows, cols, dtype=torch.int8, device=x.device),
+            torch.empty(rows, (cols + PACK_BLOCK - 1) // PACK_BLOCK, dtype=torch.float32, device=x.device))
+
+
+def pack_rows(x, num_rows=None):
+    q, scales = _packed_like(x)
+    _ck(lib.mokb_pack_rows(_p(x), _p(q), _p(scales), _p(num_rows), x.shape[0], x.shape[1], _stream()))
+    return q, scales
+
+
+def unpack_rows(q, scales, num_rows=None):
+    x = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    _ck(lib.mokb_unpack_rows(_p(q), _p(scales), _p(x), _p(num_rows), q.shape[0], q.shape[1], _stream()))
+    return x
+
+
+def swiglu_bwd_packed(gate_q, gate_scales, up_q, up_scales, d_hidden, swiglu_limit=None, row_scale=None, num_rows=None):
+    d_gate, d_up, hidden = (torch.empty_like(d_hidden) for _ in range(3))
+    row_grad = torch.empty(d_hidden.shape[0], dtype=torch.float32, device=d_hidden.device)
+    _ck(lib.mokb_swiglu_bwd_packed(_p(gate_q), _p(gate_scales), _p(up_q), _p(up_scales), _p(d_hidden), _p(d_gate), _p(d_up),
+                                   _p(hidden), _p(row_scale), _p(row_grad), _p(num_rows), d_hidden.shape[0],
+                                   d_hidden.shape[1], 0 if swiglu_limit is None else 1,
+                                   0.0 if swiglu_limit is None else float(swiglu_limit), _stream()))
+    return d_gate, d_up, hidden, row_grad
 
 
 # ----------------------------------------------------------------------------

@@ -57,6 +57,33 @@ class MoKForwardContext:
     hidden_routed: torch.Tensor | tuple[torch.Tensor, torch.Tensor]
 
 
+@dataclass(frozen=True, slots=True)
+class MoKRouterConfig:
+    """How `route` scores and weighs: see `ops.route`."""
+    topk: int
+    score: str = "softmax"           # or "sigmoid"
+    renormalize: bool = True         # a token's weights add up to `scale`
+    scale: float = 1.0
+
+
+@dataclass(frozen=True, slots=True)
+class MoKRouting:
+    top_experts: torch.Tensor                        # (T, topk) int64, as build_schedule takes them
+    router_weights: torch.Tensor                     # (T, topk) float32
+    tokens_per_expert: torch.Tensor | None           # (E,) int32, with balance
+    score_sums: torch.Tensor | None                  # (E,) float32, with balance
+
+
+@dataclass(frozen=True, slots=True)
+class MoKPackedContext:
+    """A BF16 forward context in 8 bits: pairs of q and scales (`ops.pack_rows`).  `hidden` is rebuilt from gate and up."""
+    x_routed: tuple[torch.Tensor, torch.Tensor]
+    gate_shared: tuple[torch.Tensor, torch.Tensor]
+    gate_routed: tuple[torch.Tensor, torch.Tensor]
+    up_shared: tuple[torch.Tensor, torch.Tensor]
+    up_routed: tuple[torch.Tensor, torch.Tensor]
+
+
 @dataclass(slots=True)
 class MoKWorkspace:
     group_name: str
@@ -441,10 +468,12 @@ def backward(config: MoKConfig, workspace: MoKWorkspace, schedule: MoKSchedule, 
              routed_gate_weights, routed_up_weights, routed_down_weights, swiglu_limit: float | None = None):
     """Runs the MoE backward pass (reference: mok/functional.py:652-780).  Returns (d_x, d_router_weights,
     d_routed_gate_weights, d_routed_up_weights, d_routed_down_weights, d_shared_gate_weights,
-    d_shared_up_weights, d_shared_down_weights)."""
+    d_shared_up_weights, d_shared_down_weights).  The context may be a BF16 one that `pack_context` packed; it is then left as it is."""
     validate_inputs(config, workspace, schedule, x, router_weights, grad_output)
-    if not isinstance(forward_context, MoKForwardContext):
-        raise TypeError("forward_context must be a MoKForwardContext")
+    if not isinstance(forward_context, (MoKForwardContext, MoKPackedContext)):
+        raise TypeError("forward_context must be a MoKForwardContext or a MoKPackedContext")
+    if isinstance(forward_context, MoKPackedContext) and _is_mxfp8(routed_gate_weights):
+        raise TypeError("a packed context belongs to BF16 routed weights")
     ws = workspace
     d_y_in, d_y_ptrs = _input(ws, ws.d_y_buffer, ws.d_y_buffer_ptrs, grad_output)
     x_in, x_ptrs = _input(ws, ws.x_buffer, ws.x_buffer_ptrs, x)
@@ -469,6 +498,19 @@ def backward(config: MoKConfig, workspace: MoKWorkspace, schedule: MoKSchedule, 
             ws.topk, swiglu_limit, config.bwd_num_comm_sms, config.macrobatch_size, config.minibatch_size)
         d_x_shared = outs[0]
         d_w_shared_gate, d_w_routed_gate, d_w_shared_up, d_w_routed_up, d_w_shared_down, d_w_routed_down = outs[-6:]
+    elif isinstance(ctx, MoKPackedContext):
+        outs = ops.call(
+            ops.dispatch_mlp_swiglu_combine_bwd_bf16_packed,
+            d_y_in, d_y_ptrs, ws.d_x_routed_buffer, ws.d_x_routed_buffer_ptrs,
+            weights_in, weights_ptrs, ws.d_router_weight_buffer,
+            ws.d_router_weight_buffer_ptrs,
+            shared_gate_weights, routed_gate_weights, shared_up_weights, routed_up_weights,
+            shared_down_weights, routed_down_weights,
+            *ctx.x_routed, *ctx.gate_routed, *ctx.up_routed, *ctx.gate_shared, *ctx.up_shared, x_in, x_ptrs,
+            schedule.peer_rank, schedule.peer_token_idx, schedule.num_tokens, schedule.tokens_per_expert,
+            ws.topk, swiglu_limit, config.bwd_num_comm_sms, config.macrobatch_size, config.minibatch_size)
+        d_x_shared = outs[0]
+        d_w_shared_gate, d_w_routed_gate, d_w_shared_up, d_w_routed_up, d_w_shared_down, d_w_routed_down = outs[-6:]
     else:
         outs = ops.call(
             ops.dispatch_mlp_swiglu_combine_bwd_bf16,
@@ -488,3 +530,57 @@ def backward(config: MoKConfig, workspace: MoKWorkspace, schedule: MoKSchedule, 
     d_router_weights = ws.d_router_weight_buffer.clone()
     return (d_x, d_router_weights, d_w_routed_gate, d_w_routed_up, d_w_routed_down,
             d_w_shared_gate, d_w_shared_up, d_w_shared_down)
+
+
+def route(config: MoKRouterConfig, logits: torch.Tensor, bias: torch.Tensor | None = None, *, balance: bool = False) -> MoKRouting:
+    """Picks every token's experts and their weights from the router's logits (num_tokens, num_experts), fp32 or bf16; with `balance`
+    also the figures of a load-balancing loss.  See `ops.route`."""
+    if not isinstance(config, MoKRouterConfig):
+        raise TypeError("config must be a MoKRouterConfig")
+    return MoKRouting(*ops.call(ops.route, logits, bias, config.topk, config.score, config.renormalize, config.scale, balance))
+
+
+def route_backward(config: MoKRouterConfig, logits: torch.Tensor, routing: MoKRouting, d_router_weights: torch.Tensor,
+                   d_score_sums: torch.Tensor | None = None) -> torch.Tensor:
+    """The gradient of the logits from those of the router weights (`backward`'s second result) and of the score sums."""
+    if not isinstance(config, MoKRouterConfig):
+        raise TypeError("config must be a MoKRouterConfig")
+    if not isinstance(routing, MoKRouting):
+        raise TypeError("routing must be a MoKRouting")
+    return ops.call(ops.route_bwd, logits, routing.top_experts, d_router_weights, d_score_sums, config.score, config.renormalize,
+                    config.scale)
+
+
+def forward_few_tokens(x: torch.Tensor, top_experts: torch.Tensor, router_weights: torch.Tensor,
+                       shared_gate_weights: torch.Tensor | None, shared_up_weights: torch.Tensor | None,
+                       shared_down_weights: torch.Tensor | None, routed_gate_weights, routed_up_weights, routed_down_weights,
+                       swiglu_limit: float | None = None, *, first_expert: int = 0) -> torch.Tensor:
+    """The layer's forward pass for 0 to 511 tokens (a decoding step), without workspace and schedule: x (num_tokens, hidden_size) bf16,
+    weights as in `forward` (routed ones bf16, or (fp8, scales) pairs).  It computes what this rank's experts [first_expert,
+    first_expert + num_local_experts) give; with several ranks, that hold the same tokens, the layer's output is the sum over them
+    (pass the shared weights on one rank and None on the others).  Inference only: it saves no context."""
+    weights = (routed_gate_weights, routed_up_weights, routed_down_weights)
+    if any(_is_mxfp8(w) != _is_mxfp8(weights[0]) for w in weights):
+        raise TypeError("routed weights must use the same precision representation")
+    if _is_mxfp8(weights[0]) and any(len(w) != 2 for w in weights):
+        raise ValueError("MXFP8 routed weights must be data/scale pairs")
+    (g, gs), (u, us), (d, ds) = weights if _is_mxfp8(weights[0]) else ((w, None) for w in weights)
+    return ops.call(ops.few_tokens_fwd, x, top_experts, router_weights, shared_gate_weights, shared_up_weights, shared_down_weights,
+                    g, gs, u, us, d, ds, first_expert, swiglu_limit)
+
+
+def pack_context(schedule: MoKSchedule, forward_context: MoKForwardContext) -> MoKPackedContext:
+    """A BF16 context in 8 bits, for `backward`: 1.03 bytes a value of x_routed, gate and up instead of 2, and no hidden (44 % of the bytes
+    at hidden_size = 3.5 intermediate_size).  Drop the context itself afterwards.  Only the schedule's rows are packed."""
+    if not isinstance(schedule, MoKSchedule):
+        raise TypeError("schedule must be a MoKSchedule")
+    if not isinstance(forward_context, MoKForwardContext):
+        raise TypeError("forward_context must be a MoKForwardContext")
+    c = forward_context
+    if _is_mxfp8(c.gate_routed):
+        raise TypeError("an MXFP8 context is in 8 bits already")
+    rows = schedule.num_tokens
+    return MoKPackedContext(
+        x_routed=ops.call(ops.pack_rows, c.x_routed, rows), gate_shared=ops.call(ops.pack_rows, c.gate_shared, None),
+        gate_routed=ops.call(ops.pack_rows, c.gate_routed, rows), up_shared=ops.call(ops.pack_rows, c.up_shared, None),
+        up_routed=ops.call(ops.pack_rows, c.up_routed, rows))

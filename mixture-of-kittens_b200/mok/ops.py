@@ -476,3 +476,12 @@ from .ops_mxfp8 import (  # noqa: E402,F401
     dispatch_mlp_swiglu_combine_fwd_mxfp8,
     recompute_forward_context_mxfp8,
 )
+from .ops_tokens import (  # noqa: E402,F401
+    dispatch_mlp_swiglu_combine_bwd_bf16_packed,
+    few_tokens_fwd,
+    pack_rows,
+    route,
+    route_bwd,
+    swiglu_bwd_packed,
+    unpack_rows,
+)
