@@ -8,12 +8,13 @@
 // are the 128-row side of tcgen05.mma (A, streamed by TMA) and the tokens of an expert its narrow side (N = 16 .. 128), and what is
 // tuned is how evenly the stream of weights is spread over the SMs.
 //
-// Three launches, tied by programmatic dependent launch (a kernel's set-up, and the down projection's first weights, go ahead of the
+// Four launches, tied by programmatic dependent launch (a kernel's set-up, and the down projection's first weights, go ahead of the
 // end of the kernel before it):
 //   plan   one block: the tokens of every local expert, in `units` of at most 128 columns; clears the counters.  MXFP8: further blocks
 //          quantise x (E4M3 + E8M0 along the hidden axis, what the layer's pull does).
 //   gate/up  tile = 128 gate rows and the 128 up rows beside them (two accumulators, so a thread holds both): hidden = silu(g) * u
-//   down     tile = 256 rows of W_down; a token's result is summed by whoever finishes its last expert (below)
+//   down     tile = 256 rows of W_down; fp32 results, one row per route
+//   sum      y[t] = shared + sum over k = 0, 1, .. of w[t, k] * result, rounded once
 // Work is cut by stages of the contraction, not by tiles: the stages of all tiles are numbered through and every CTA takes an equal,
 // contiguous range (7 experts of 1408 x 5120 are 77 gate/up tiles on 148 SMs).  A tile that falls to several CTAs is summed by the one
 // that finishes last, in the order of the contraction, from fp32 partial sums in global memory: nobody waits, so calls on several
@@ -23,7 +24,8 @@
 //   warp 0     TMA producer: weights (two 128-row boxes of 128 bytes per stage) and, MXFP8, their scale tiles
 //   warp 1     MMA issuer
 //   warps 2-5  epilogue
-//   warps 6-7  the tokens' rows: gathered with 16-byte cp.async into the swizzled layout, visible to the tensor cores after a proxy fence
+//   warps 6-7  the tokens' rows: gathered with 16-byte cp.async into the swizzled layout; the copies themselves arrive on the stage's
+//              barrier, so as many stages are under way as the ring holds, and the MMA issuer makes them visible to the tensor cores
 #include "common.cuh"
 #include "mxfp8_codec.cuh"
 
@@ -37,7 +39,6 @@ constexpr int SF_BYTES = 3 * 512;               // MXFP8: the scale tiles of bot
 constexpr int kMaxStages = 8;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kCtrlBytes = 1024;                // barriers, flags, row lists
-constexpr int kLag = 2;                         // cp.async groups in flight behind the newest
 // No CTA takes fewer stages than this: below it, what a tile's partial sums cost is more than a stage's load.
 constexpr int kMinStages = 4;
 constexpr int kPlanThreads = 1024;
@@ -58,8 +59,7 @@ struct Work {
     Unit* units;
     int32_t* slot_token;      // [T * K] token of a slot; slots are numbered expert by expert
     int32_t* pos;             // [T * K] slot of a route, -1: not of this rank, or without weight
-    int32_t* need;            // [T] results that a token is summed from
-    int32_t* counters;        // tickets of the split tiles [2][SMs], then results counted per token and 256 columns [T][H / 256]
+    int32_t* counters;        // [2][SMs] tickets of the tiles that several CTAs share
     uint8_t* xq;              // MXFP8: [T, H] E4M3
     uint32_t* xs;             // MXFP8: [T, H / 128] four scale bytes each
     uint8_t* hid_q;           // MXFP8: [T * K, I]
@@ -75,7 +75,6 @@ inline int column_cap(int T, bool mx) {
     return n < unit_columns(mx) ? n : unit_columns(mx);
 }
 inline int max_units(int T, int K, bool mx) { return T * K + T / column_cap(T, mx) + 2; }      // a routed unit has a route; shared ones
-__host__ __device__ inline int counter_words(int T, int H, int sms) { return 2 * sms + T * (H / 256); }
 
 inline size_t carve_few(Work* w, void* base, int T, int H, int I, int K, bool mx, int sms) {
     char* const p0 = static_cast<char*>(base);
@@ -87,8 +86,7 @@ inline size_t carve_few(Work* w, void* base, int T, int H, int I, int K, bool mx
     v.units = reinterpret_cast<Unit*>(take(sizeof(Unit) * max_units(T, K, mx)));
     v.slot_token = reinterpret_cast<int32_t*>(take(R * 4));
     v.pos = reinterpret_cast<int32_t*>(take(R * 4));
-    v.need = reinterpret_cast<int32_t*>(take(static_cast<size_t>(T) * 4));
-    v.counters = reinterpret_cast<int32_t*>(take(4 * static_cast<size_t>(counter_words(T, H, sms))));
+    v.counters = reinterpret_cast<int32_t*>(take(static_cast<size_t>(sms) * 8));
     v.xq = reinterpret_cast<uint8_t*>(take(mx ? static_cast<size_t>(T) * H : 0));
     v.xs = reinterpret_cast<uint32_t*>(take(mx ? static_cast<size_t>(T) * (H / 128) * 4 : 0));
     v.hid_q = reinterpret_cast<uint8_t*>(take(mx ? R * I : 0));
@@ -127,8 +125,11 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// arrives on the barrier (one of its expected arrivals) once this thread's copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // 32 lanes x 16 consecutive fp32 columns of tensor memory
 __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&f)[16]) {
@@ -206,7 +207,7 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
     extern __shared__ int32_t count[];           // [E], then the experts' first slots
     const int NT = p.col_cap, R = p.T * p.K;      // (an expert named twice by a token can have more routes than there are tokens)
     for (int i = t0; i < p.E; i += kPlanThreads) count[i] = 0;
-    for (int i = t0; i < counter_words(p.T, p.H, p.sms); i += kPlanThreads) p.w.counters[i] = 0;
+    for (int i = t0; i < 2 * p.sms; i += kPlanThreads) p.w.counters[i] = 0;
     __syncthreads();
     for (int j = t0; j < R; j += kPlanThreads) {
         const int64_t e = p.top_experts[j] - p.first_expert;
@@ -240,12 +241,6 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
         const int slot = count[p.top_experts[j] - p.first_expert] + rank;
         p.w.pos[j] = slot;
         p.w.slot_token[slot] = j / p.K;
-    }
-    __syncthreads();
-    for (int t = t0; t < p.T; t += kPlanThreads) {
-        int n = p.shared;
-        for (int k = 0; k < p.K; ++k) n += p.w.pos[t * p.K + k] >= 0 ? 1 : 0;
-        p.w.need[t] = n;
     }
 }
 
@@ -322,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(full_bar(s), 1 + kLoaderWarps);       // the weights' bytes, and one arrival per loader warp
+            mbar_init(full_bar(s), 1 + 32 * kLoaderWarps);  // the weights' bytes, and an arrival per lane of the loader warps
             mbar_init(empty_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
@@ -347,10 +342,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    if (!DOWN) {
-        grid_dep_wait();              // the plan
-        grid_dep_launch();
-    }
+    if (!DOWN) grid_dep_wait();       // the plan
+    grid_dep_launch();
     // DOWN: the gate/up kernel let this one start after it had seen the plan finished, so the plan may be read at once (through L2, past
     // lines that an earlier call may have left in L1); only what that kernel itself writes has to be waited for.
     const int n_units = __ldcg(p.w.header), n_shared = __ldcg(p.w.header + 1);
@@ -413,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                 const uint32_t idesc = (npad >> 3) << 17 | (128u >> 4) << 24 | (mx ? 1u << 23 : 1u << 4 | 1u << 7 | 1u << 10);
                 for (int k = g.k0; k < g.k1; ++k) {
                     if (!mbar_wait(full_bar(s), ph, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT)) { ok = false; break; }
+                    fence_proxy_async_smem();          // the tokens' rows came through the generic proxy
                     tc_fence_after();
                     const uint32_t a = smem_base + s * data_bytes;
                     const uint64_t a0 = make_smem_desc(a, 16, 1024), a1 = make_smem_desc(a + A_BYTES / 2, 16, 1024);
@@ -445,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
         // ------------------------------------------------------------ the tokens' rows
         if (DOWN) grid_dep_wait();            // hidden
         const int lw = warp - 6, chunk = lane & 7, sub = lane >> 3;      // a lane: 16 bytes of one row of four
-        int s = 0, arrive_s = 0, behind = 0;
+        int s = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (int64_t at = s_begin; ok && at < s_end;) {
@@ -473,39 +467,16 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                     for (int n = lw * 4 + (lane >> 2) * 8 + (lane & 3); n < unit.n; n += 64)
                         cp_async_4(sf + static_cast<uint32_t>((n & 31) * 16 + (n >> 5) * 4), scales + static_cast<int64_t>(row_list[n]) * kt + k);
                 }
-                cp_async_commit();
-                // a stage is handed over when the copies issued kLag stages later are on their way
-                if (behind == kLag) {
-                    cp_async_wait<kLag>();
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full_bar(arrive_s));
-                    if (++arrive_s == S) arrive_s = 0;
-                } else {
-                    ++behind;
-                }
+                cp_async_arrive(full_bar(s));
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
         }
-        cp_async_wait<0>();
-        fence_proxy_async_smem();
-        __syncwarp();
-        for (; ok && behind > 0; --behind) {
-            if (lane == 0) mbar_arrive(full_bar(arrive_s));
-            if (++arrive_s == S) arrive_s = 0;
-        }
+        cp_async_wait_all();
     } else {
         // ------------------------------------------------------------ epilogue
         const int quarter = warp & 3, row = quarter * 32 + lane, et = threadIdx.x - 64;
         const float limit = p.has_limit ? p.limit : __int_as_float(0x7f800000);
         const size_t part_stride = static_cast<size_t>(p.col_cap) * 128;      // one accumulator's partial sums
-        if (DOWN) {
-            grid_dep_wait();                   // (the counters were cleared by the plan; y and the results are written from here on)
-            // tokens that nothing is computed for
-            for (int t = cta; t < p.T; t += p.sms)
-                if (__ldcg(p.w.need + t) == 0)
-                    for (int c = et; c < p.H / 8; c += 128) reinterpret_cast<uint4*>(p.y + static_cast<size_t>(t) * p.H)[c] = make_uint4(0, 0, 0, 0);
-        }
         int local = 0;
         for (int64_t at = s_begin; at < s_end; ++local) {
             const Segment g = segment_at(st, at, s_end);
@@ -596,42 +567,6 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tempty_bar(buf));
             }
-            if (DOWN) {
-                // Count the unit's tokens; whoever brings a token's count to its number of results sums them.
-                __threadfence();
-                epilogue_sync();
-                for (int n0 = (warp - 2) * 32; n0 < unit.n; n0 += 128) {
-                    int token = -1;
-                    bool last = false;
-                    if (n0 + lane < unit.n) {
-                        token = sh ? unit.slot0 + n0 + lane : __ldcg(p.w.slot_token + unit.slot0 + n0 + lane);
-                        int32_t* const done = p.w.counters + 2 * p.sms + token * st.blocks + blk;
-                        last = atomicAdd(done, 1) + 1 == __ldcg(p.w.need + token);
-                    }
-                    __threadfence();
-                    __syncwarp();
-                    for (unsigned todo = __ballot_sync(0xffffffffu, last); todo; todo &= todo - 1) {
-                        const int t = __shfl_sync(0xffffffffu, token, __ffs(todo) - 1);
-                        const int col = blk * 256 + lane * 8;
-                        float sum[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
-                        auto add = [&](int64_t r, float w) {
-                            const float4* const v = reinterpret_cast<const float4*>(p.w.yr + r * p.H + col);
-                            const float4 a = __ldcg(v), b = __ldcg(v + 1);
-                            sum[0] += w * a.x; sum[1] += w * a.y; sum[2] += w * a.z; sum[3] += w * a.w;
-                            sum[4] += w * b.x; sum[5] += w * b.y; sum[6] += w * b.z; sum[7] += w * b.w;
-                        };
-                        if (p.shared) add(p.T * p.K + t, 1.0f);
-                        for (int k = 0; k < p.K; ++k) {
-                            const int slot = __ldcg(p.w.pos + t * p.K + k);
-                            if (slot >= 0) add(slot, __ldg(p.weights + t * p.K + k));
-                        }
-                        *reinterpret_cast<uint4*>(p.y + static_cast<size_t>(t) * p.H + col) =
-                            make_uint4(pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3]), pack_bf16(sum[4], sum[5]), pack_bf16(sum[6], sum[7]));
-                    }
-                }
-            }
         }
     }
 
@@ -650,6 +585,55 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- sum
+// A warp per 256 columns of a token: the shared expert's result, then the routes in order, eight at a time in flight.
+__global__ void __launch_bounds__(128) few_sum_kernel(const FewParams p) {
+    grid_dep_wait();
+    const int lane = threadIdx.x & 31, blocks = p.H / 256;
+    const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (item >= p.T * blocks) return;
+    const int t = item / blocks, col = (item - t * blocks) * 256 + lane * 8;
+    float sum[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+    if (p.shared) {
+        const float4* const v = reinterpret_cast<const float4*>(p.w.yr + static_cast<int64_t>(p.T * p.K + t) * p.H + col);
+        const float4 a = __ldcg(v), b = __ldcg(v + 1);
+        sum[0] = a.x; sum[1] = a.y; sum[2] = a.z; sum[3] = a.w; sum[4] = b.x; sum[5] = b.y; sum[6] = b.z; sum[7] = b.w;
+    }
+    for (int k0 = 0; k0 < p.K; k0 += 32) {
+        const int mine = k0 + lane < p.K ? __ldcg(p.w.pos + t * p.K + k0 + lane) : -1;
+        const float weight = mine >= 0 ? __ldg(p.weights + t * p.K + k0 + lane) : 0.0f;
+        unsigned todo = __ballot_sync(0xffffffffu, mine >= 0);
+        while (todo) {
+            float4 a[8], b[8];
+            float w[8];
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                w[i] = 0.0f;
+                if (todo) {
+                    const int k = __ffs(todo) - 1;
+                    todo &= todo - 1;
+                    const float4* const v = reinterpret_cast<const float4*>(p.w.yr + static_cast<int64_t>(__shfl_sync(0xffffffffu, mine, k)) * p.H + col);
+                    w[i] = __shfl_sync(0xffffffffu, weight, k);
+                    a[i] = __ldcg(v);
+                    b[i] = __ldcg(v + 1);
+                    ++n;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (i >= n) break;
+                sum[0] += w[i] * a[i].x; sum[1] += w[i] * a[i].y; sum[2] += w[i] * a[i].z; sum[3] += w[i] * a[i].w;
+                sum[4] += w[i] * b[i].x; sum[5] += w[i] * b[i].y; sum[6] += w[i] * b[i].z; sum[7] += w[i] * b[i].w;
+            }
+        }
+    }
+    *reinterpret_cast<uint4*>(p.y + static_cast<size_t>(t) * p.H + col) =
+        make_uint4(pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3]), pack_bf16(sum[4], sum[5]), pack_bf16(sum[6], sum[7]));
+}
+
 template <class... Args>
 int launch_after(void (*kernel)(Args...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
     cudaLaunchConfig_t cfg = {};
@@ -664,6 +648,18 @@ int launch_after(void (*kernel)(Args...), unsigned grid, unsigned threads, size_
     cfg.numAttrs = 1;
     MOKB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
     note_launch();
+    return MOKB_OK;
+}
+
+// once per device: the attribute belongs to the device's context
+int allow_shared_memory() {
+    static bool done[64] = {false};
+    int dev = -1;
+    MOKB_CUDA(cudaGetDevice(&dev));
+    if (dev >= 0 && dev < 64 && __atomic_load_n(&done[dev], __ATOMIC_RELAXED)) return MOKB_OK;
+    MOKB_CUDA(cudaFuncSetAttribute(few_product_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+    MOKB_CUDA(cudaFuncSetAttribute(few_product_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+    if (dev >= 0 && dev < 64) __atomic_store_n(&done[dev], true, __ATOMIC_RELAXED);
     return MOKB_OK;
 }
 
@@ -741,12 +737,12 @@ extern "C" int mokb_few_tokens_fwd(const mokb_few_tokens_args* a, void* stream_)
         MOKB_TRY(make_tmap_2d(&dn.scale0, a->w_routed_down_sc, 4, 128, tiles, 512, 128, 1));
         dn.scale1 = dn.scale0;
     }
-    MOKB_CUDA(cudaFuncSetAttribute(few_product_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
-    MOKB_CUDA(cudaFuncSetAttribute(few_product_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+    MOKB_TRY(allow_shared_memory());
     const int pieces = p.T * ((H + 1023) / 1024), quant_blocks = mx ? (pieces + 31) / 32 : 0;
     few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), kPlanThreads, static_cast<size_t>(p.E) * 4, stream>>>(p);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
     MOKB_TRY(launch_after(few_product_kernel<false>, static_cast<unsigned>(p.sms), kThreads, smem, stream, gu, p));
-    return launch_after(few_product_kernel<true>, static_cast<unsigned>(p.sms), kThreads, smem, stream, dn, p);
+    MOKB_TRY(launch_after(few_product_kernel<true>, static_cast<unsigned>(p.sms), kThreads, smem, stream, dn, p));
+    return launch_after(few_sum_kernel, static_cast<unsigned>((p.T * (H / 256) + 3) / 4), 128, 0, stream, p);
 }

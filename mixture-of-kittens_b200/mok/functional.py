@@ -581,6 +581,6 @@ def pack_context(schedule: MoKSchedule, forward_context: MoKForwardContext) -> M
         raise TypeError("an MXFP8 context is in 8 bits already")
     rows = schedule.num_tokens
     return MoKPackedContext(
-        x_routed=ops.call(ops.pack_rows, c.x_routed, rows), gate_shared=ops.call(ops.pack_rows, c.gate_shared, None),
-        gate_routed=ops.call(ops.pack_rows, c.gate_routed, rows), up_shared=ops.call(ops.pack_rows, c.up_shared, None),
-        up_routed=ops.call(ops.pack_rows, c.up_routed, rows))
+        x_routed=ops.pack_rows(c.x_routed, rows), gate_shared=ops.pack_rows(c.gate_shared),
+        gate_routed=ops.pack_rows(c.gate_routed, rows), up_shared=ops.pack_rows(c.up_shared),
+        up_routed=ops.pack_rows(c.up_routed, rows))

@@ -198,7 +198,7 @@ def _check_packed(name: str, q, scales, device=None) -> tuple[int, int]:
 
 
 @_ops._op("mok::pack_rows", mutates_args=())
-def pack_rows(x: torch.Tensor, num_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+def pack_rows_op(x: torch.Tensor, num_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 [rows, columns] -> q int8 and scales [rows, ceil(columns / 128)] fp32: x ~ q * scale, one scale per 128 values of a row,
     off by half a step of max|x| / 127 at most.  With `num_rows` (int32 [1] on the device, e.g. a schedule's num_tokens) only the
     first num_rows rows are packed and the others are left unwritten."""
@@ -211,7 +211,7 @@ def pack_rows(x: torch.Tensor, num_rows: torch.Tensor | None = None) -> tuple[to
 
 
 @_ops._op("mok::unpack_rows", mutates_args=())
-def unpack_rows(q: torch.Tensor, scales: torch.Tensor, num_rows: torch.Tensor | None = None) -> torch.Tensor:
+def unpack_rows_op(q: torch.Tensor, scales: torch.Tensor, num_rows: torch.Tensor | None = None) -> torch.Tensor:
     """What `pack_rows` kept, as bf16."""
     _check_packed("q", q, scales)
     _check_num_rows(num_rows, q.device)
@@ -219,7 +219,7 @@ def unpack_rows(q: torch.Tensor, scales: torch.Tensor, num_rows: torch.Tensor | 
 
 
 @_ops._op("mok::swiglu_bwd_packed", mutates_args=())
-def swiglu_bwd_packed(
+def swiglu_bwd_packed_op(
     gate_q: torch.Tensor,
     gate_scales: torch.Tensor,
     up_q: torch.Tensor,
@@ -240,6 +240,23 @@ def swiglu_bwd_packed(
         _check_cuda("row_scale", row_scale, F32, shape[:1], gate_q.device)
     _check_num_rows(num_rows, gate_q.device)
     return _C.swiglu_bwd_packed(gate_q, gate_scales, up_q, up_scales, d_hidden, swiglu_limit, row_scale, num_rows)
+
+
+# The three above are called as they are, also many times a step, so the public names take the short way that `call` knows.
+def pack_rows(x, num_rows=None):
+    return _ops.call(pack_rows_op, x, num_rows)
+
+
+def unpack_rows(q, scales, num_rows=None):
+    return _ops.call(unpack_rows_op, q, scales, num_rows)
+
+
+def swiglu_bwd_packed(gate_q, gate_scales, up_q, up_scales, d_hidden, swiglu_limit=None, row_scale=None, num_rows=None):
+    return _ops.call(swiglu_bwd_packed_op, gate_q, gate_scales, up_q, up_scales, d_hidden, swiglu_limit, row_scale, num_rows)
+
+
+for _f, _o in ((pack_rows, pack_rows_op), (unpack_rows, unpack_rows_op), (swiglu_bwd_packed, swiglu_bwd_packed_op)):
+    _f.__doc__ = _ops._EAGER[_o][0].__doc__
 
 
 @_ops._op(
