@@ -23,8 +23,8 @@
 //
 //   warp 0     TMA producer: weights (two 128-row boxes of 128 bytes per stage) and, MXFP8, their scale tiles
 //   warp 1     MMA issuer
-//   warps 2-5  epilogue
-//   warps 6-7  the tokens' rows: gathered with 16-byte cp.async into the swizzled layout; the copies themselves arrive on the stage's
+//   warps 2-9  epilogue
+//   warps 10-  the tokens' rows: gathered with 16-byte cp.async into the swizzled layout; the copies themselves arrive on the stage's
 //              barrier, so as many stages are under way as the ring holds, and the MMA issuer makes them visible to the tensor cores
 #include "common.cuh"
 #include "mxfp8_codec.cuh"
@@ -32,25 +32,28 @@
 namespace mokb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kLoaderWarps = 2;
+constexpr int kEpilogueWarps = 8;               // two per quarter of tensor memory
+constexpr int kLoaderWarps = 4;
+constexpr int kThreads = 32 * (2 + kEpilogueWarps + kLoaderWarps);
 constexpr int A_BYTES = 2 * 128 * 128;          // two boxes of 128 rows x 128 bytes
 constexpr int SF_BYTES = 3 * 512;               // MXFP8: the scale tiles of both boxes and of the tokens
 constexpr int kMaxStages = 8;
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int kCtrlBytes = 1024;                // barriers, flags, row lists
+constexpr int kCtrlBytes = 512 + kLoaderWarps * 512;      // barriers, flags; a row list per loader warp
 // No CTA takes fewer stages than this: below it, what a tile's partial sums cost is more than a stage's load.
 constexpr int kMinStages = 4;
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kPlanThreadsSmall = 256, kKept = 4;
 
 // columns of a unit: two accumulators, double buffered, fill the 512 columns of tensor memory; MXFP8 keeps 32 of them for the scales
 __host__ __device__ constexpr int unit_columns(bool mx) { return mx ? 112 : 128; }
 
+// An expert's routes are cut into units of equal size; the tiles of its units alternate (rows first, then units), so that a second
+// unit finds the weights in L2.
 struct Unit {
     int expert;       // -1: the shared expert
     int n;            // columns (tokens)
     int slot0;        // first slot; shared: first token
-    int unused;
+    int place;        // number among the expert's units << 16 | how many those are
 };
 
 // The call's work area.
@@ -117,7 +120,7 @@ struct FewMaps {                       // by-value kernel argument: the two boxe
 
 __device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory"); }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -145,10 +148,10 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, float (&f)[16]) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- plan
-// Exclusive block-wide prefix sum of two counts per thread (1024 threads).
+// Exclusive block-wide prefix sum of two counts per thread.
 __device__ __forceinline__ int2 block_scan(int2 v, int2* total) {
-    __shared__ int2 warp_sum[32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __shared__ int2 warp_sum[kPlanThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int2 inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -157,20 +160,16 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* total) {
     }
     if (lane == 31) warp_sum[warp] = inc;
     __syncthreads();
-    if (warp == 0) {
-        int2 s = warp_sum[lane];
+    int2 s = lane < warps ? warp_sum[lane] : make_int2(0, 0);       // every warp scans the sums for itself
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
-            if (lane >= o) { s.x += a; s.y += b; }
-        }
-        warp_sum[lane] = s;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, s.x, o), b = __shfl_up_sync(0xffffffffu, s.y, o);
+        if (lane >= o) { s.x += a; s.y += b; }
     }
+    *total = make_int2(__shfl_sync(0xffffffffu, s.x, 31), __shfl_sync(0xffffffffu, s.y, 31));
+    const int bx = __shfl_sync(0xffffffffu, s.x, max(warp - 1, 0)), by = __shfl_sync(0xffffffffu, s.y, max(warp - 1, 0));
     __syncthreads();
-    *total = warp_sum[31];
-    const int2 before = warp ? warp_sum[warp - 1] : make_int2(0, 0);
-    __syncthreads();
-    return make_int2(before.x + inc.x - v.x, before.y + inc.y - v.y);
+    return make_int2((warp ? bx : 0) + inc.x - v.x, (warp ? by : 0) + inc.y - v.y);
 }
 
 // Block 0 lays out the routes; with MXFP8 weights blocks 1.. quantise x, a warp per 1024 values of a row at a time.
@@ -180,8 +179,8 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
     const int t0 = threadIdx.x;
     if (blockIdx.x > 0) {
         const int lane = t0 & 31, per_row = (p.H + 1023) / 1024;
-        const int pieces = p.T * per_row, stride = (gridDim.x - 1) * (kPlanThreads / 32);
-        for (int i = (blockIdx.x - 1) * (kPlanThreads / 32) + (t0 >> 5); i < pieces; i += stride) {
+        const int warps = blockDim.x >> 5, pieces = p.T * per_row, stride = (gridDim.x - 1) * warps;
+        for (int i = (blockIdx.x - 1) * warps + (t0 >> 5); i < pieces; i += stride) {
             const int t = i / per_row, c0 = (i - t * per_row) * 1024 + lane * 32;      // a lane: one block of 32 values
             if (c0 >= p.H) continue;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(p.x + static_cast<size_t>(t) * p.H + c0);
@@ -204,29 +203,45 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
         }
         return;
     }
-    extern __shared__ int32_t count[];           // [E], then the experts' first slots
-    const int NT = p.col_cap, R = p.T * p.K;      // (an expert named twice by a token can have more routes than there are tokens)
-    for (int i = t0; i < p.E; i += kPlanThreads) count[i] = 0;
-    for (int i = t0; i < 2 * p.sms; i += kPlanThreads) p.w.counters[i] = 0;
-    __syncthreads();
-    for (int j = t0; j < R; j += kPlanThreads) {
+    extern __shared__ int32_t count[];           // [E] routes, then the experts' first slots
+    const int NT = p.col_cap, R = p.T * p.K, n_threads = blockDim.x;      // (an expert named twice by a token can have more routes than there are tokens)
+    // a thread keeps its first kKept routes in registers between the two passes; further ones leave their number in `pos`
+    int expert[kKept], number[kKept];
+    auto expert_of = [&](int j) {                // -1: not of this rank, or without weight (a weight that is NaN counts)
         const int64_t e = p.top_experts[j] - p.first_expert;
-        const bool mine = e >= 0 && e < p.E && p.weights[j] != 0.0f;      // (a weight that is NaN counts)
-        p.w.pos[j] = mine ? atomicAdd(&count[e], 1) : -1;                 // number among the expert's routes
+        return e >= 0 && e < p.E && p.weights[j] != 0.0f ? static_cast<int>(e) : -1;
+    };
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) expert[i] = t0 + i * n_threads < R ? expert_of(t0 + i * n_threads) : -1;
+    for (int i = t0; i < p.E; i += n_threads) count[i] = 0;
+    for (int i = t0; i < 2 * p.sms; i += n_threads) p.w.counters[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) number[i] = expert[i] >= 0 ? atomicAdd(&count[expert[i]], 1) : 0;
+    for (int j = t0 + kKept * n_threads; j < R; j += n_threads) {
+        const int e = expert_of(j);
+        p.w.pos[j] = e >= 0 ? atomicAdd(&count[e], 1) : -1;
     }
     __syncthreads();
     const int shared_units = p.shared ? (p.T + NT - 1) / NT : 0;
-    if (t0 < shared_units) p.w.units[t0] = Unit{-1, min(NT, p.T - t0 * NT), t0 * NT, 0};
+    if (t0 < shared_units) {
+        const int lo = t0 * p.T / shared_units, hi = (t0 + 1) * p.T / shared_units;
+        p.w.units[t0] = Unit{-1, hi - lo, lo, t0 << 16 | shared_units};
+    }
     int2 carry = make_int2(0, shared_units);     // slots, units
-    for (int e0 = 0; e0 < p.E; e0 += kPlanThreads) {
+    for (int e0 = 0; e0 < p.E; e0 += n_threads) {
         const int e = e0 + t0;
         const int n = e < p.E ? count[e] : 0;
         int2 total;
-        int2 at = block_scan(make_int2(n, (n + NT - 1) / NT), &total);
+        const int cuts = (n + NT - 1) / NT;
+        int2 at = block_scan(make_int2(n, cuts), &total);
         at.x += carry.x;
         at.y += carry.y;
         if (e < p.E) count[e] = at.x;
-        for (int c = 0; c < n; c += NT) p.w.units[at.y++] = Unit{e, min(NT, n - c), at.x + c, 0};
+        for (int c = 0; c < cuts; ++c) {
+            const int lo = static_cast<int>(static_cast<int64_t>(c) * n / cuts), hi = static_cast<int>(static_cast<int64_t>(c + 1) * n / cuts);
+            p.w.units[at.y + c] = Unit{e, hi - lo, at.x + lo, c << 16 | cuts};
+        }
         carry.x += total.x;
         carry.y += total.y;
     }
@@ -235,10 +250,18 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
         p.w.header[1] = shared_units;
     }
     __syncthreads();
-    for (int j = t0; j < R; j += kPlanThreads) {
-        const int rank = p.w.pos[j];
-        if (rank < 0) continue;
-        const int slot = count[p.top_experts[j] - p.first_expert] + rank;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i) {
+        const int j = t0 + i * n_threads;
+        if (j >= R) break;
+        const int slot = expert[i] >= 0 ? count[expert[i]] + number[i] : -1;
+        p.w.pos[j] = slot;
+        if (slot >= 0) p.w.slot_token[slot] = j / p.K;
+    }
+    for (int j = t0 + kKept * n_threads; j < R; j += n_threads) {
+        const int n = p.w.pos[j];
+        if (n < 0) continue;
+        const int slot = count[p.top_experts[j] - p.first_expert] + n;
         p.w.pos[j] = slot;
         p.w.slot_token[slot] = j / p.K;
     }
@@ -287,9 +310,20 @@ __device__ __forceinline__ Segment segment_at(const Stream& st, int64_t s, int64
     g.k1 = left < g.ks ? static_cast<int>(left) : g.ks;
     return g;
 }
-__device__ __forceinline__ Unit load_unit(const FewParams& p, int u) {
-    const int4 v = __ldcg(reinterpret_cast<const int4*>(p.w.units) + u);
-    return Unit{v.x, v.y, v.z, 0};
+// The unit of a tile and the tile's number among the unit's row blocks.
+__device__ __forceinline__ Unit unit_of(const FewParams& p, int tile, int blocks, int* blk) {
+    const int4* const units = reinterpret_cast<const int4*>(p.w.units);
+    int u = tile / blocks;
+    int4 v = __ldcg(units + u);
+    *blk = tile - u * blocks;
+    const int cuts = v.w & 0xffff;
+    if (cuts > 1) {
+        u -= v.w >> 16;                                   // the expert's first unit
+        const int in = tile - u * blocks;
+        *blk = in / cuts;
+        v = __ldcg(units + u + (in - *blk * cuts));
+    }
+    return Unit{v.x, v.y, v.z, v.w};
 }
 
 template <bool DOWN>
@@ -311,18 +345,17 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
     uint8_t* const ctrl = smem_gen + ctrl_off;
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(ctrl + 8 * (2 * kMaxStages + 4));
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * kMaxStages + 4) + 4);
-    volatile int* const last_flag = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * kMaxStages + 4) + 8);
-    int32_t* const row_list = reinterpret_cast<int32_t*>(ctrl + 512);          // [128]: the row that column n is read from
+    volatile int* const vote = reinterpret_cast<volatile int*>(ctrl + 8 * (2 * kMaxStages + 4) + 8);      // [2], used in turn
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
-            mbar_init(full_bar(s), 1 + 32 * kLoaderWarps);  // the weights' bytes, and an arrival per lane of the loader warps
+            mbar_init(full_bar(s), 1 + 32);                 // the weights' bytes, and an arrival per lane of the stage's loader warp
             mbar_init(empty_bar(s), 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(tfull_bar(a), 1);
-            mbar_init(tempty_bar(a), 4);                    // one arrival per epilogue warp
+            mbar_init(tempty_bar(a), kEpilogueWarps);
         }
         *abort_flag = 0;
         fence_barrier_init();
@@ -364,8 +397,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
             for (int64_t at = s_begin; ok && at < s_end;) {
                 const Segment g = segment_at(st, at, s_end);
                 at += g.k1 - g.k0;
-                const int u = g.tile / st.blocks, blk = g.tile - u * st.blocks;
-                const int expert = load_unit(p, u).expert;
+                int blk;
+                const int expert = unit_of(p, g.tile, st.blocks, &blk).expert;
                 const bool sh = expert < 0, mx = p.mx && !sh;
                 const CUtensorMap* const m0 = sh ? &maps.shared0 : &maps.routed0;
                 const CUtensorMap* const m1 = sh ? &maps.shared1 : &maps.routed1;
@@ -395,7 +428,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
             for (int64_t at = s_begin; ok && at < s_end; ++local) {
                 const Segment g = segment_at(st, at, s_end);
                 at += g.k1 - g.k0;
-                const Unit unit = load_unit(p, g.tile / st.blocks);
+                int blk;
+                const Unit unit = unit_of(p, g.tile, st.blocks, &blk);
                 const bool mx = p.mx && unit.expert >= 0;
                 const uint32_t npad = static_cast<uint32_t>((unit.n + 15) & ~15);
                 const int buf = local & 1;
@@ -435,103 +469,129 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                 if (ok) umma_commit(tfull_bar(buf));
             }
         }
-    } else if (warp >= 6) {
+    } else if (warp >= 2 + kEpilogueWarps) {
         // ------------------------------------------------------------ the tokens' rows
         if (DOWN) grid_dep_wait();            // hidden
-        const int lw = warp - 6, chunk = lane & 7, sub = lane >> 3;      // a lane: 16 bytes of one row of four
-        int s = 0;
+        // Every fourth stage is this warp's as a whole: an arrival per lane and stage costs less than one per lane of four warps.
+        const int lw = warp - 2 - kEpilogueWarps, chunk = lane & 7, sub = lane >> 3;      // a lane: 16 bytes of one row of four
+        int32_t* const rows = reinterpret_cast<int32_t*>(ctrl + 512 + lw * 512);      // [128]: the row that column n is read from
+        int s = 0, turn = 0;
         uint32_t ph = 0;
         bool ok = true;
         for (int64_t at = s_begin; ok && at < s_end;) {
             const Segment g = segment_at(st, at, s_end);
             at += g.k1 - g.k0;
-            const Unit unit = load_unit(p, g.tile / st.blocks);
+            int blk;
+            const Unit unit = unit_of(p, g.tile, st.blocks, &blk);
             const bool sh = unit.expert < 0, mx = p.mx && !sh;
-            // this warp's rows: groups of four, every other one
             __syncwarp();
-            for (int n = lw * 4 + (lane >> 2) * 8 + (lane & 3); n < unit.n; n += 64)
-                row_list[n] = DOWN ? unit.slot0 + n + (sh ? p.T * p.K : 0) : sh ? unit.slot0 + n : __ldcg(p.w.slot_token + unit.slot0 + n);
+            for (int n = lane; n < unit.n; n += 32)
+                rows[n] = DOWN ? unit.slot0 + n + (sh ? p.T * p.K : 0) : sh ? unit.slot0 + n : __ldcg(p.w.slot_token + unit.slot0 + n);
             __syncwarp();
             const int64_t row_bytes = (DOWN ? p.I : p.H) * (mx ? 1 : 2);
-            const uint8_t* const src = DOWN ? (mx ? p.w.hid_q : reinterpret_cast<const uint8_t*>(p.w.hid))
-                                            : (mx ? p.w.xq : reinterpret_cast<const uint8_t*>(p.x));
+            const uint8_t* const src = (DOWN ? (mx ? p.w.hid_q : reinterpret_cast<const uint8_t*>(p.w.hid))
+                                             : (mx ? p.w.xq : reinterpret_cast<const uint8_t*>(p.x))) + chunk * 16;
             const uint32_t* const scales = DOWN ? reinterpret_cast<const uint32_t*>(p.w.hid_s) : p.w.xs;
             const int kt = (DOWN ? p.I : p.H) / 128;
             for (int k = g.k0; k < g.k1; ++k) {
-                if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT)) { ok = false; break; }
-                const uint32_t dst = smem_base + s * data_bytes + A_BYTES;
-                for (int n = lw * 4 + sub; n < unit.n; n += 8)
-                    cp_async_16(dst + n * 128u + static_cast<uint32_t>((chunk ^ (n & 7)) << 4), src + row_list[n] * row_bytes + k * 128 + chunk * 16);
-                if (mx) {
-                    const uint32_t sf = sf_base + s * SF_BYTES + 1024;
-                    for (int n = lw * 4 + (lane >> 2) * 8 + (lane & 3); n < unit.n; n += 64)
-                        cp_async_4(sf + static_cast<uint32_t>((n & 31) * 16 + (n >> 5) * 4), scales + static_cast<int64_t>(row_list[n]) * kt + k);
+                if (turn == lw) {
+                    if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT)) { ok = false; break; }
+                    const uint32_t dst = smem_base + s * data_bytes + A_BYTES;
+                    const uint8_t* const from = src + k * 128;
+#pragma unroll 4
+                    for (int n = sub; n < unit.n; n += 4)
+                        cp_async_16(dst + n * 128u + static_cast<uint32_t>((chunk ^ (n & 7)) << 4), from + rows[n] * row_bytes);
+                    if (mx) {
+                        const uint32_t sf = sf_base + s * SF_BYTES + 1024;
+                        for (int n = lane; n < unit.n; n += 32)
+                            cp_async_4(sf + static_cast<uint32_t>((n & 31) * 16 + (n >> 5) * 4), scales + static_cast<int64_t>(rows[n]) * kt + k);
+                    }
+                    cp_async_arrive(full_bar(s));
                 }
-                cp_async_arrive(full_bar(s));
+                if (++turn == kLoaderWarps) turn = 0;
                 if (++s == S) { s = 0; ph ^= 1u; }
             }
         }
         cp_async_wait_all();
     } else {
         // ------------------------------------------------------------ epilogue
-        const int quarter = warp & 3, row = quarter * 32 + lane, et = threadIdx.x - 64;
+        // A warp: 32 rows (the quarter of tensor memory that it may read) and every other 16 columns.
+        const int quarter = warp & 3, row = quarter * 32 + lane, first_col = ((warp - 2) >> 2) * 16, et = threadIdx.x - 64;
         const float limit = p.has_limit ? p.limit : __int_as_float(0x7f800000);
         const size_t part_stride = static_cast<size_t>(p.col_cap) * 128;      // one accumulator's partial sums
-        int local = 0;
+        // slot 1: the tile begins in CTA q (and ends in a later one); slot 0: it began in an earlier one
+        auto part_of = [&](int q, int c_lo) { return p.w.part + (static_cast<size_t>(q) * 2 + (q == c_lo ? 1 : 0)) * 2 * part_stride + row; };
+        int local = 0, votes = 0;
         for (int64_t at = s_begin; at < s_end; ++local) {
             const Segment g = segment_at(st, at, s_end);
             at += g.k1 - g.k0;
-            const int u = g.tile / st.blocks, blk = g.tile - u * st.blocks;
-            const Unit unit = load_unit(p, u);
+            int blk;
+            const Unit unit = unit_of(p, g.tile, st.blocks, &blk);
             const bool sh = unit.expert < 0;
             const int buf = local & 1;
+            // Is everybody else through with the tile?  Asked ahead of this CTA's own end: mostly it comes last (the next CTA began with
+            // the tile's other part), and then its sums never leave tensor memory.
+            const int c_lo = g.k0 == 0 && g.k1 == g.ks ? cta : st.owner(g.first), c_hi = c_lo == cta && g.k1 == g.ks ? cta : st.owner(g.first + g.ks - 1);
+            int32_t* const ticket = p.w.counters + (DOWN ? p.sms : 0) + c_lo;
             if (!mbar_wait(tfull_bar(buf), (local >> 1) & 1u, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT)) break;
             tc_fence_after();
             const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * 2 * acc_cols, t1 = t0 + acc_cols;
-            const bool whole = g.k0 == 0 && g.k1 == g.ks;
-            int c_lo = cta, c_hi = cta;
-            if (!whole) {
-                c_lo = st.owner(g.first);
-                c_hi = st.owner(g.first + g.ks - 1);
-                // slot 1: the tile begins in this CTA (and ends in a later one); slot 0: it began in an earlier one
-                float* const mine = p.w.part + (static_cast<size_t>(cta) * 2 + (cta == c_lo ? 1 : 0)) * 2 * part_stride + row;
-                for (int c = 0; c < unit.n; c += 16) {
-                    float a[16], b[16];
-                    tmem_ld_32x16(t0 + c, a);
-                    tmem_ld_32x16(t1 + c, b);
+            bool mine_in_tmem = true;
+            if (c_lo != c_hi) {
+                // (a word of `vote` is written again only after a later barrier than the one before it was read)
+                if (et == 0) vote[votes & 1] = ld_acquire_gpu(ticket) == c_hi - c_lo ? 1 : 0;
+                epilogue_sync();
+                if (!vote[votes++ & 1]) {
+                    mine_in_tmem = false;
+                    float* const mine = part_of(cta, c_lo);
+                    for (int c = first_col; c < unit.n; c += 32) {
+                        float a[16], b[16];
+                        tmem_ld_32x16(t0 + c, a);
+                        tmem_ld_32x16(t1 + c, b);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (c + j >= unit.n) break;
-                        mine[(c + j) * 128] = a[j];
-                        mine[part_stride + (c + j) * 128] = b[j];
+                        for (int j = 0; j < 16; ++j)
+                            if (c + j < unit.n) {
+                                mine[(c + j) * 128] = a[j];
+                                mine[part_stride + (c + j) * 128] = b[j];
+                            }
                     }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(tempty_bar(buf));
+                    __threadfence();
+                    epilogue_sync();
+                    if (et == 0) vote[votes & 1] = atomicAdd(ticket, 1) == c_hi - c_lo ? 1 : 0;
+                    epilogue_sync();
+                    if (!vote[votes++ & 1]) continue;
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(tempty_bar(buf));
-                __threadfence();
-                epilogue_sync();
-                if (et == 0) *last_flag = atomicAdd(p.w.counters + (DOWN ? p.sms : 0) + c_lo, 1) == c_hi - c_lo ? 1 : 0;
-                epilogue_sync();
-                if (!*last_flag) continue;
                 __threadfence();
             }
-            for (int c = 0; c < unit.n; c += 16) {
+            for (int c = first_col; c < unit.n; c += 32) {
                 float a[16], b[16];
-                if (whole) {
+                if (c_lo == c_hi) {
                     tmem_ld_32x16(t0 + c, a);
                     tmem_ld_32x16(t1 + c, b);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 16; ++j) a[j] = b[j] = 0.0f;
-                    for (int q = c_lo; q <= c_hi; ++q) {      // in the order of the contraction
-                        const float* const theirs = p.w.part + (static_cast<size_t>(q) * 2 + (q == c_lo ? 1 : 0)) * 2 * part_stride + row;
+                    for (int q = c_lo; q <= c_hi; ++q) {      // in the order of the contraction, whoever is last
+                        float x[16], y[16];
+                        if (q == cta && mine_in_tmem) {
+                            tmem_ld_32x16(t0 + c, x);
+                            tmem_ld_32x16(t1 + c, y);
+                        } else {
+                            const float* const theirs = part_of(q, c_lo);
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (c + j < unit.n) {
-                                a[j] += __ldcg(theirs + (c + j) * 128);
-                                b[j] += __ldcg(theirs + part_stride + (c + j) * 128);
+                            for (int j = 0; j < 16; ++j) {
+                                x[j] = c + j < unit.n ? __ldcg(theirs + (c + j) * 128) : 0.0f;
+                                y[j] = c + j < unit.n ? __ldcg(theirs + part_stride + (c + j) * 128) : 0.0f;
                             }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            a[j] += x[j];
+                            b[j] += y[j];
+                        }
                     }
                 }
 #pragma unroll
@@ -544,9 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                         dst[128] = b[j];
                     } else {
                         const float gate = fminf(a[j], limit), up = fminf(fmaxf(b[j], -limit), limit);
-                        // (a NaN of the product must come out as one: fminf drops it)
-                        float h = gate / (1.0f + __expf(-gate)) * up;
-                        if (a[j] != a[j] || b[j] != b[j]) h = a[j] + b[j];
+                        // the approximate reciprocal of a quarter of the denominator: of all of it, it would be zero for gates near -88
+                        float h = __fdividef(0.25f * gate, fmaf(0.25f, __expf(-gate), 0.25f)) * up;
+                        if (a[j] != a[j] || b[j] != b[j]) h = a[j] + b[j];      // (the clamps drop a NaN)
                         if (p.mx && !sh) {
                             // the warp's 32 rows are one block of the hidden axis
                             const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(h) & 0x7fffffffu);
@@ -562,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                     }
                 }
             }
-            if (whole) {
+            if (mine_in_tmem) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(tempty_bar(buf));
@@ -738,8 +798,10 @@ extern "C" int mokb_few_tokens_fwd(const mokb_few_tokens_args* a, void* stream_)
         dn.scale1 = dn.scale0;
     }
     MOKB_TRY(allow_shared_memory());
-    const int pieces = p.T * ((H + 1023) / 1024), quant_blocks = mx ? (pieces + 31) / 32 : 0;
-    few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), kPlanThreads, static_cast<size_t>(p.E) * 4, stream>>>(p);
+    // few routes: fewer threads to start and to wait for
+    const int plan_threads = p.T * p.K <= kPlanThreadsSmall && p.E <= 2 * kPlanThreadsSmall ? kPlanThreadsSmall : kPlanThreads;
+    const int pieces = p.T * ((H + 1023) / 1024), quant_blocks = mx ? (pieces + plan_threads / 32 - 1) / (plan_threads / 32) : 0;
+    few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), plan_threads, static_cast<size_t>(p.E) * 4, stream>>>(p);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
     MOKB_TRY(launch_after(few_product_kernel<false>, static_cast<unsigned>(p.sms), kThreads, smem, stream, gu, p));

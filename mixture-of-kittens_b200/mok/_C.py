@@ -588,7 +588,7 @@ def few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w
     E, I = w_routed_gate.shape[:2]
     K = top_experts.shape[1]
     mx = int(scales is not None)
-    y = torch.empty(T, H, dtype=torch.bfloat16, device=x.device)
+    y = torch.empty_like(x)
     work = torch.empty(lib.mokb_few_tokens_workspace_bytes(T, H, I, K, mx), dtype=torch.uint8, device=x.device)
     a = FewTokensArgs(T, H, I, E, K, first_expert, mx, 0 if swiglu_limit is None else 1,
                       0.0 if swiglu_limit is None else float(swiglu_limit), _p(x), _p(top_experts), _p(router_weights),

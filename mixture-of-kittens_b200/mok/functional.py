@@ -559,12 +559,13 @@ def forward_few_tokens(x: torch.Tensor, top_experts: torch.Tensor, router_weight
     weights as in `forward` (routed ones bf16, or (fp8, scales) pairs).  It computes what this rank's experts [first_expert,
     first_expert + num_local_experts) give; with several ranks, that hold the same tokens, the layer's output is the sum over them
     (pass the shared weights on one rank and None on the others).  Inference only: it saves no context."""
-    weights = (routed_gate_weights, routed_up_weights, routed_down_weights)
-    if any(_is_mxfp8(w) != _is_mxfp8(weights[0]) for w in weights):
-        raise TypeError("routed weights must use the same precision representation")
-    if _is_mxfp8(weights[0]) and any(len(w) != 2 for w in weights):
-        raise ValueError("MXFP8 routed weights must be data/scale pairs")
-    (g, gs), (u, us), (d, ds) = weights if _is_mxfp8(weights[0]) else ((w, None) for w in weights)
+    g, u, d, gs, us, ds = routed_gate_weights, routed_up_weights, routed_down_weights, None, None, None
+    if _is_mxfp8(g) or _is_mxfp8(u) or _is_mxfp8(d):
+        if not (_is_mxfp8(g) and _is_mxfp8(u) and _is_mxfp8(d)):
+            raise TypeError("routed weights must use the same precision representation")
+        if not len(g) == len(u) == len(d) == 2:
+            raise ValueError("MXFP8 routed weights must be data/scale pairs")
+        (g, gs), (u, us), (d, ds) = g, u, d
     return ops.call(ops.few_tokens_fwd, x, top_experts, router_weights, shared_gate_weights, shared_up_weights, shared_down_weights,
                     g, gs, u, us, d, ds, first_expert, swiglu_limit)
 

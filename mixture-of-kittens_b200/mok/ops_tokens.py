@@ -36,6 +36,11 @@ def _check_cuda(name: str, t: torch.Tensor, dtype, shape=None, device=None, cont
         raise ValueError(f"{name} must be contiguous")
 
 
+def _plain(t, dtype, shape, device) -> bool:
+    """What `_check_cuda` accepts, asked in one go: the detailed checks only have to name what is wrong."""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()
+
+
 def _check_limit(swiglu_limit) -> None:
     if swiglu_limit is not None and (type(swiglu_limit) not in (int, float) or not swiglu_limit >= 0):
         raise ValueError("swiglu_limit must be None or a non-negative number")
@@ -150,26 +155,29 @@ def few_tokens_fwd(
     K = top_experts.shape[1]
     if type(first_expert) is not int or not 0 <= first_expert < 2 ** 31:
         raise ValueError("first_expert must be a non-negative integer")
-    _check_limit(swiglu_limit)
+    if swiglu_limit is not None:
+        _check_limit(swiglu_limit)
     _check_cuda("x", x, BF16)
     dev = x.device
-    _check_cuda("top_experts", top_experts, I64, (T, K), dev)
-    _check_cuda("router_weights", router_weights, F32, (T, K), dev)
     scales = (w_routed_gate_sc, w_routed_up_sc, w_routed_down_sc)
-    mx = scales[0] is not None
-    if any((s is not None) != mx for s in scales):
-        raise ValueError("the scales of the routed weights go together")
-    for name, w, sc, rows, cols in (("w_routed_gate", w_routed_gate, scales[0], I, H), ("w_routed_up", w_routed_up, scales[1], I, H),
-                                    ("w_routed_down", w_routed_down, scales[2], H, I)):
-        _check_cuda(name, w, F8 if mx else BF16, (E, rows, cols), dev)
-        if mx:
-            _check_cuda(f"{name}_sc", sc, torch.uint8, _sc_shape(E * rows, cols), dev)
     shared = (w_shared_gate, w_shared_up, w_shared_down)
-    if any((w is None) != (shared[0] is None) for w in shared):
-        raise ValueError("the shared expert's weights go together")
-    if shared[0] is not None:
-        for name, w, shape in zip(("w_shared_gate", "w_shared_up", "w_shared_down"), shared, ((I, H), (I, H), (H, I))):
-            _check_cuda(name, w, BF16, shape, dev)
+    mx = scales[0] is not None
+    table = [("top_experts", top_experts, I64, (T, K)), ("router_weights", router_weights, F32, (T, K)),
+             ("w_routed_gate", w_routed_gate, F8 if mx else BF16, (E, I, H)), ("w_routed_up", w_routed_up, F8 if mx else BF16, (E, I, H)),
+             ("w_routed_down", w_routed_down, F8 if mx else BF16, (E, H, I))]
+    if mx or scales[1] is not None or scales[2] is not None:
+        if any(s is None for s in scales):
+            raise ValueError("the scales of the routed weights go together")
+        table += [(f"{name}_sc", sc, torch.uint8, _sc_shape(E * rows, cols)) for name, sc, rows, cols in
+                  zip(("w_routed_gate", "w_routed_up", "w_routed_down"), scales, (I, I, H), (H, H, I))]
+    if shared[0] is not None or shared[1] is not None or shared[2] is not None:
+        if any(w is None for w in shared):
+            raise ValueError("the shared expert's weights go together")
+        table += [("w_shared_gate", w_shared_gate, BF16, (I, H)), ("w_shared_up", w_shared_up, BF16, (I, H)),
+                  ("w_shared_down", w_shared_down, BF16, (H, I))]
+    for name, t, dtype, shape in table:
+        if not _plain(t, dtype, shape, dev):
+            _check_cuda(name, t, dtype, shape, dev)
     if T == 0:
         return torch.empty_like(x)
     return _C.few_tokens_fwd(x, top_experts, router_weights, *shared, w_routed_gate, w_routed_up, w_routed_down,
