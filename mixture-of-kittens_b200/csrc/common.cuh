@@ -274,6 +274,29 @@ __device__ __forceinline__ bool index_ok(const IndexGuard& g, int idx, int kind,
     return false;
 }
 
+// ---- programmatic dependent launch: a kernel launched with launch_after() (below) may start once every block of the kernel before it has
+// called grid_dep_launch() or ended; what it needs of that kernel's results it reads after grid_dep_wait(), which returns when that kernel
+// is complete.  (Both do nothing in a kernel that is launched otherwise.)
+__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... Args>
+inline int launch_after(void (*kernel)(Args...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    MOKB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
+    note_launch();
+    return MOKB_OK;
+}
+
 // ---- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* t) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(t)) : "memory");

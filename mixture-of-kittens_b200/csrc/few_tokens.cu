@@ -118,8 +118,6 @@ struct FewMaps {                       // by-value kernel argument: the two boxe
     CUtensorMap routed0, routed1, shared0, shared1, scale0, scale1;
 };
 
-__device__ __forceinline__ void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void epilogue_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpilogueWarps) : "memory"); }
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
@@ -647,12 +645,18 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
 
 // ---------------------------------------------------------------------------------------------------------------- sum
 // A warp per 256 columns of a token: the shared expert's result, then the routes in order, eight at a time in flight.
+// (The plan was complete before the down projection could start, so the routes' slots are read ahead of the wait.)
 __global__ void __launch_bounds__(128) few_sum_kernel(const FewParams p) {
-    grid_dep_wait();
     const int lane = threadIdx.x & 31, blocks = p.H / 256;
     const int item = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (item >= p.T * blocks) return;
-    const int t = item / blocks, col = (item - t * blocks) * 256 + lane * 8;
+    const bool live = item < p.T * blocks;
+    const int t = live ? item / blocks : 0, col = (item - t * blocks) * 256 + lane * 8;
+    auto slot_of = [&](int k) { return k < p.K ? __ldcg(p.w.pos + t * p.K + k) : -1; };
+    auto weight_of = [&](int k) { return k < p.K ? __ldg(p.weights + t * p.K + k) : 0.0f; };
+    int mine = slot_of(lane);
+    float weight = weight_of(lane);
+    grid_dep_wait();
+    if (!live) return;
     float sum[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
@@ -662,8 +666,10 @@ __global__ void __launch_bounds__(128) few_sum_kernel(const FewParams p) {
         sum[0] = a.x; sum[1] = a.y; sum[2] = a.z; sum[3] = a.w; sum[4] = b.x; sum[5] = b.y; sum[6] = b.z; sum[7] = b.w;
     }
     for (int k0 = 0; k0 < p.K; k0 += 32) {
-        const int mine = k0 + lane < p.K ? __ldcg(p.w.pos + t * p.K + k0 + lane) : -1;
-        const float weight = mine >= 0 ? __ldg(p.weights + t * p.K + k0 + lane) : 0.0f;
+        if (k0 > 0) {
+            mine = slot_of(k0 + lane);
+            weight = weight_of(k0 + lane);
+        }
         unsigned todo = __ballot_sync(0xffffffffu, mine >= 0);
         while (todo) {
             float4 a[8], b[8];
@@ -692,23 +698,6 @@ __global__ void __launch_bounds__(128) few_sum_kernel(const FewParams p) {
     }
     *reinterpret_cast<uint4*>(p.y + static_cast<size_t>(t) * p.H + col) =
         make_uint4(pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3]), pack_bf16(sum[4], sum[5]), pack_bf16(sum[6], sum[7]));
-}
-
-template <class... Args>
-int launch_after(void (*kernel)(Args...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    MOKB_CUDA(cudaLaunchKernelEx(&cfg, kernel, args...));
-    note_launch();
-    return MOKB_OK;
 }
 
 // once per device: the attribute belongs to the device's context

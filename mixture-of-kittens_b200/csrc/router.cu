@@ -7,17 +7,24 @@
 // so that a token always has topk different experts, as the schedule wants.  Ties go to the lowest index, picks come in falling order.
 //
 // One warp per token; a lane holds PER of its logits in registers, so forward and backward read them once (a pick's own logit is read
-// again by the lane that writes its weight: a cache hit).  A pick is a maximum over the lanes of an order-preserving 32-bit key and a
-// minimum over the indices that have it.  Bound by instruction issue at long micro-batches: a pick costs about 3 PER + 20 instructions
-// a warp.
+// again by the lane that writes its weight: a cache hit).  The next token's row is on its way while one is worked on.
+//
+// Picking: a key is a 32-bit number of the logits' order whose low bits give way to the expert's index (inverted: the lowest index is the
+// largest key), so that one maximum over the warp is a pick, and no two keys are alike.  Every lane keeps its two largest; only a lane that
+// has given both looks for its next two.  For bf16 logits nothing is lost by that.  For fp32 ones the order of two that agree in all other
+// bits is open: where that happens between neighbours in the order of the picks (the first that is left out among them), the row is done
+// again by key and index.  With a bias the keys are s + bias, and two of them a rounding apart must not change places with how exp is
+// evaluated: the order is that of the sums worked out in 64 bits and rounded to 32.  They too are first picked in 32 bits, and the row is
+// done again in 64 where neighbours are nearer than the error of that.
+// (16384 x 256, 8 picks: 28 us looking through all keys for every pick, 19 with keys and indices apart.)
+//
+// Bound by instruction issue at long micro-batches.
 #include <float.h>
 
 #include "common.cuh"
 
 namespace mokb {
 namespace {
-
-constexpr int kClosedKey = 1;          // below every number's key; 0: taken, or no expert
 
 struct RouteParams {
     const void* logits;
@@ -43,7 +50,7 @@ template <bool BF16> __device__ __forceinline__ float load_one(const void* p, in
     return BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
-// This lane's logits of one row; experts beyond E and closed ones come as -inf, +inf as the largest number.
+// This lane's logits of one row as they are; -inf beyond E.
 template <int PER, bool BF16, bool VEC>
 __device__ __forceinline__ void load_row(const RouteParams& p, int64_t row, int lane, float (&v)[PER]) {
     const int64_t base = row * p.ld;
@@ -70,64 +77,125 @@ __device__ __forceinline__ void load_row(const RouteParams& p, int64_t row, int 
             if (e < p.E) v[i] = load_one<BF16>(p.logits, base + e);
         }
     }
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] = fminf(v[i] == v[i] ? v[i] : -INFINITY, FLT_MAX);
 }
+// NaN closes an expert like -inf; +inf counts as the largest number
+__device__ __forceinline__ float clean(float v) { return fminf(v == v ? v : -INFINITY, FLT_MAX); }
 template <bool BF16>
-__device__ __forceinline__ float clean_logit(const RouteParams& p, int64_t row, int e) {
-    const float v = load_one<BF16>(p.logits, row * p.ld + e);
-    return fminf(v == v ? v : -INFINITY, FLT_MAX);
-}
+__device__ __forceinline__ float load_clean(const RouteParams& p, int64_t row, int e) { return clean(load_one<BF16>(p.logits, row * p.ld + e)); }
 
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
 }
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-    return x;
-}
-
-// number -> key of the same order (0 and -0 alike); -inf is closed
+// number -> key of the same order (0 and -0 alike), and back
 __device__ __forceinline__ uint32_t order_key(float v) {
     const uint32_t b = __float_as_uint(v + 0.0f);
     return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-__device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
+constexpr uint32_t kClosedKey = 0x007fffffu;          // order_key(-inf)
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float sigmoid(float l) { return __fdividef(1.0f, 1.0f + exp2_approx(-kLog2E * l)); }      // (-inf: 0)
 
-// The scores of one row, in place of its logits.  `top`: the row's largest logit (softmax).
+// exp(l - top) of a row's logits, in place, and their sum (SIGMOID: the scores themselves).  Closed ones give 0; a row that is closed as a
+// whole has top = -inf.  The exponent is one rounding of a product and one of a sum off: |top| + |l - top| half units.
 template <int PER, bool SIGMOID>
-__device__ __forceinline__ void scores(float (&v)[PER], float top, float* inv_total) {
+__device__ __forceinline__ float exponentials(float (&v)[PER], float top) {
     if (SIGMOID) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = sigmoid(v[i]);          // (-inf: 0)
-        *inv_total = 1.0f;
-        return;
+        for (int i = 0; i < PER; ++i) v[i] = sigmoid(v[i]);
+        return 1.0f;
     }
     float total = 0.0f;
+    const float at = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        v[i] = v[i] == -INFINITY ? 0.0f : expf(v[i] - top);          // (a row that is closed as a whole: top is -inf too)
+        v[i] = exp2_approx((v[i] - at) * kLog2E);
         total += v[i];
     }
-    total = warp_sum(total);
-    *inv_total = total > 0.0f ? 1.0f / total : 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) v[i] *= *inv_total;
+    return warp_sum(total);
 }
 template <bool SIGMOID>
 __device__ __forceinline__ float score_of(float l, float top, float inv_total) {
-    return SIGMOID ? sigmoid(l) : l == -INFINITY ? 0.0f : expf(l - top) * inv_total;
+    return SIGMOID ? sigmoid(l) : l == -INFINITY ? 0.0f : exp2_approx((l - top) * kLog2E) * inv_total;
 }
 
-constexpr int route_threads(int per) { return per <= 8 ? 512 : 256; }
+constexpr int index_bits(int per) { return per == 4 ? 7 : per == 8 ? 8 : per == 16 ? 9 : 10; }
+
+// The topk largest keys, indices in their low bits, in falling order: lane k returns the k-th one's expert.  CHECK: one more is looked for,
+// and *open says whether the order of two neighbours is not settled (closed experts always are): keys that differ only in the index, or
+// (BIASED) sums that are nearer than their errors.
+template <int PER, bool CHECK, bool BIASED>
+__device__ __forceinline__ int pick(const uint32_t (&key)[PER], int K, int lane, bool* open) {
+    constexpr int B = index_bits(PER);
+    uint32_t b1, b2, mine = 0u, before = 0u;      // b1, b2: this lane's two largest that are not taken
+    int cached = 2;
+    auto look = [&](uint32_t below) {
+        b1 = b2 = 0u;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t k = key[i] < below ? key[i] : 0u;
+            b2 = max(b2, min(b1, k));
+            b1 = max(b1, k);
+        }
+    };
+    look(0xffffffffu);
+    if (CHECK) *open = false;
+    const int rounds = CHECK ? K + 1 : K;
+    for (int k = 0; k < rounds; ++k) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, b1);
+        if (lane == k) mine = top;
+        if (CHECK && k > 0 && (top >> B) > (kClosedKey >> B)) {
+            if (BIASED) {
+                // both keys lost up to 2^(B - 23) of their size to the index
+                const float hi = key_value(before), lo = key_value(top);
+                *open = *open || hi - lo <= 1e-6f + (1e-6f + 2.0f / (1 << (22 - B))) * fmaxf(fabsf(hi), fabsf(lo));
+            } else {
+                *open = *open || ((before ^ top) >> B) == 0u;
+            }
+        }
+        before = top;
+        if (b1 == top) {
+            b1 = b2;
+            if (--cached == 0) {
+                look(top);
+                cached = 2;
+            }
+        }
+    }
+    return ((1 << B) - 1) - static_cast<int>(mine & ((1u << B) - 1u));
+}
+// The same by key and index, for rows whose order that leaves open.
+template <int PER, bool VEC>
+__device__ __forceinline__ int pick_by_key_and_index(uint32_t (&key)[PER], int K, int lane) {
+    int mine = 0;
+#pragma unroll 1
+    for (int k = 0; k < K; ++k) {
+        uint32_t best = 0u;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (key[i] > best) { best = key[i]; at = i; }            // (a lane's experts ascend with i)
+        const uint32_t top = __reduce_max_sync(0xffffffffu, best);
+        const int e = __reduce_min_sync(0xffffffffu, best == top ? expert_of<VEC>(at, lane) : 0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (expert_of<VEC>(i, lane) == e) key[i] = 0u;
+        if (lane == k) mine = e;
+    }
+    return mine;
+}
+
+constexpr int route_threads(int per) { return per <= 8 ? 256 : 128; }
+constexpr int route_blocks_per_sm(int per) { return per <= 4 ? 5 : per <= 8 ? 4 : per <= 16 ? 5 : 3; }
 
 template <int PER, bool BF16, bool VEC, bool SIGMOID>
-__global__ void __launch_bounds__(route_threads(PER)) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) route_kernel(const RouteParams p) {
     extern __shared__ int32_t sm[];          // balance: [E] counts, [E] sums
+    grid_dep_launch();                       // (the blocks that add up the load figures come in as these leave)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const bool balance = p.part_count != nullptr;
     float* const sums = reinterpret_cast<float*>(sm + p.E);
@@ -138,43 +206,66 @@ __global__ void __launch_bounds__(route_threads(PER)) route_kernel(const RoutePa
         for (int i = 0; i < PER; ++i) acc[i] = 0.0f;
         __syncthreads();
     }
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp; row < p.T; row += static_cast<int64_t>(gridDim.x) * warps) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp;
+    float next[PER];
+    if (row < p.T) load_row<PER, BF16, VEC>(p, row, lane, next);
+    for (; row < p.T; row += step) {
         float v[PER];
-        load_row<PER, BF16, VEC>(p, row, lane, v);
-        uint32_t key[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = clean(next[i]);
+        if (row + step < p.T) load_row<PER, BF16, VEC>(p, row + step, lane, next);
+        constexpr uint32_t kIndex = (1u << index_bits(PER)) - 1u;
+        uint32_t key[PER];                   // 0: no expert
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int e = expert_of<VEC>(i, lane);
-            if (SIGMOID && p.bias) {
-                // Two scores a rounding apart must not change places with how exp is evaluated: in 64 bits, compared as 32-bit numbers.
-                if (e < p.E) key[i] = v[i] == -INFINITY ? kClosedKey : order_key(static_cast<float>(1.0 / (1.0 + exp(-static_cast<double>(v[i]))) + static_cast<double>(p.bias[e])));
-                else key[i] = 0u;
-            } else {
-                key[i] = e >= p.E ? 0u : v[i] == -INFINITY ? kClosedKey : order_key(v[i]);
+            float order = v[i];
+            if (SIGMOID && p.bias && order > -INFINITY && e < p.E) order = sigmoid(order) + __ldg(p.bias + e);
+            key[i] = e >= p.E ? 0u : (order_key(order) & ~kIndex) | (kIndex - static_cast<uint32_t>(e));
+        }
+        int mine;                            // lane k: the k-th pick
+        if (SIGMOID && p.bias) {
+            // s in 32 bits: an exp (off by some 2 + 1.2 |l| units in the last place; s (1 - s) <= 1/4 and |l| s (1 - s) < 0.23 of that), a sum
+            // and a quotient: below 3e-7.  s + bias and the 32-bit form of the exact sum are rounded once each.  Two neighbours that are
+            // more than 1e-6 (1 + |s + bias|) apart are in order.
+            bool open;
+            mine = pick<PER, true, true>(key, p.K, lane, &open);
+            if (open) {
+#pragma unroll 1
+                for (int i = 0; i < PER; ++i) {
+                    const int e = expert_of<VEC>(i, lane);
+                    uint32_t exact = 0u;
+                    if (e < p.E) {
+                        const double l = load_clean<BF16>(p, row, e);
+                        exact = l == -INFINITY ? kClosedKey : order_key(static_cast<float>(1.0 / (1.0 + exp(-l)) + static_cast<double>(p.bias[e])));
+                    }
+#pragma unroll
+                    for (int j = 0; j < PER; ++j)
+                        if (j == i) key[j] = exact;
+                }
+                mine = pick_by_key_and_index<PER, VEC>(key, p.K, lane);
+            }
+        } else if (BF16) {
+            mine = pick<PER, false, false>(key, p.K, lane, nullptr);
+        } else {
+            bool open;
+            mine = pick<PER, true, false>(key, p.K, lane, &open);
+            if (open) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) key[i] = expert_of<VEC>(i, lane) < p.E ? order_key(v[i]) : 0u;
+                mine = pick_by_key_and_index<PER, VEC>(key, p.K, lane);
             }
         }
-        int mine = 0;                        // lane k: the k-th pick
-        for (int k = 0; k < p.K; ++k) {
-            uint32_t best = 0u;
-            int at = 0;
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (key[i] > best) { best = key[i]; at = i; }        // (a lane's experts ascend with i)
-            const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-            const int e = __reduce_min_sync(0xffffffffu, best == top ? expert_of<VEC>(at, lane) : 0x7fffffff);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (expert_of<VEC>(i, lane) == e) key[i] = 0u;
-            if (lane == k) mine = e;
-        }
-        const float l = lane < p.K ? clean_logit<BF16>(p, row, mine) : -INFINITY;
+        const float l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
         float inv_total = 1.0f, top = 0.0f;
         if (!SIGMOID) top = __shfl_sync(0xffffffffu, l, 0);          // the first pick has the largest logit
         if (balance || (!SIGMOID && !p.renormalize)) {
-            scores<PER, SIGMOID>(v, top, &inv_total);
+            const float total = exponentials<PER, SIGMOID>(v, top);
+            if (!SIGMOID) inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
             if (balance) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) acc[i] += v[i];
+                for (int i = 0; i < PER; ++i) acc[i] += v[i] * inv_total;
                 if (lane < p.K && l > -INFINITY) atomicAdd(&sm[mine], 1);
             }
         }
@@ -207,23 +298,32 @@ __global__ void __launch_bounds__(route_threads(PER)) route_kernel(const RoutePa
     }
 }
 
-// Adds up the blocks' load figures: 32 experts per block, 32 threads each, in a fixed order.
-__global__ void __launch_bounds__(1024) route_reduce_kernel(const int32_t* __restrict__ part_count, const float* __restrict__ part_sum,
-                                                            int blocks, int E, int32_t* __restrict__ count, float* __restrict__ sum) {
-    __shared__ int32_t c_sm[32][33];
-    __shared__ float s_sm[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, e = blockIdx.x * 32 + x;
+// Adds up the blocks' load figures in a fixed order: 8 experts per block, 128 threads each.
+__global__ void __launch_bounds__(1024) route_reduce_kernel(const int32_t* part_count, const float* part_sum, int blocks, int E, int32_t* count, float* sum) {
+    __shared__ int32_t c_sm[32][9];
+    __shared__ float s_sm[32][9];
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3, e = blockIdx.x * 8 + x;
     int32_t c = 0;
     float s = 0.0f;
-    if (e < E)
-        for (int b = y; b < blocks; b += 32) {
-            c += part_count[static_cast<int64_t>(b) * E + e];
-            s += part_sum[static_cast<int64_t>(b) * E + e];
+    grid_dep_wait();
+    if (e < E) {
+#pragma unroll 8
+        for (int b = y; b < blocks; b += 128) {
+            c += __ldcg(part_count + static_cast<int64_t>(b) * E + e);
+            s += __ldcg(part_sum + static_cast<int64_t>(b) * E + e);
         }
-    c_sm[y][x] = c;
-    s_sm[y][x] = s;
+    }
+#pragma unroll
+    for (int o = 8; o < 32; o <<= 1) {          // the four rows of a warp
+        c += __shfl_xor_sync(0xffffffffu, c, o);
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+    }
+    if ((threadIdx.x & 31) < 8) {
+        c_sm[threadIdx.x >> 5][x] = c;
+        s_sm[threadIdx.x >> 5][x] = s;
+    }
     __syncthreads();
-    if (y == 0 && e < E) {
+    if (threadIdx.x < 8 && e < E) {
         c = 0;
         s = 0.0f;
 #pragma unroll
@@ -235,50 +335,88 @@ __global__ void __launch_bounds__(1024) route_reduce_kernel(const int32_t* __res
 
 // d s_k from d w_k: scale * d w_k, or with `renormalize` scale * (d w_k - sum_j share_j d w_j) / norm; plus d_score_sums on every
 // expert.  Then d l = s (d s - sum s d s) (softmax) or d s * s (1 - s) (sigmoid).
+// The picks' part of d s goes to the lanes that hold those experts through shared memory: a row of E numbers per warp that holds
+// d_score_sums (or zeros) between tokens.
 template <int PER, bool BF16, bool VEC, bool SIGMOID>
-__global__ void __launch_bounds__(route_threads(PER)) route_bwd_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) route_bwd_kernel(const RouteParams p) {
+    extern __shared__ __align__(16) float rows_sm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp; row < p.T; row += static_cast<int64_t>(gridDim.x) * warps) {
-        float v[PER];
-        load_row<PER, BF16, VEC>(p, row, lane, v);
-        int mine = -1;
-        float dw = 0.0f, l = -INFINITY;
+    float* const ds_sm = rows_sm + warp * PER * 32;
+    uint8_t* const tag_sm = reinterpret_cast<uint8_t*>(rows_sm + warps * PER * 32) + warp * PER * 32;      // who wrote an expert's number last
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int e = expert_of<VEC>(i, lane);
+        ds_sm[e] = p.d_score_sums && e < p.E ? __ldg(p.d_score_sums + e) : 0.0f;
+    }
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp;
+    float next[PER];
+    int64_t next_pick = -1;
+    float next_dw = 0.0f;
+    auto fetch = [&](int64_t r) {
+        load_row<PER, BF16, VEC>(p, r, lane, next);
         if (lane < p.K) {
-            const int64_t e = p.picked[row * p.K + lane];
-            if (e >= 0 && e < p.E) {                       // anything else has no logit
-                mine = static_cast<int>(e);
-                dw = p.d_weights[row * p.K + lane] * p.scale;
-                l = clean_logit<BF16>(p, row, mine);
-            }
+            next_pick = p.picked[r * p.K + lane];
+            next_dw = p.d_weights[r * p.K + lane];
         }
-        float top = 0.0f, inv_total;
+    };
+    if (row < p.T) fetch(row);
+    for (; row < p.T; row += step) {
+        float v[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = clean(next[i]);
+        const int mine = next_pick >= 0 && next_pick < p.E ? static_cast<int>(next_pick) : -1;      // anything else has no logit
+        const float dw = mine >= 0 ? next_dw * p.scale : 0.0f;
+        const float l = mine >= 0 ? load_clean<BF16>(p, row, mine) : -INFINITY;
+        if (row + step < p.T) fetch(row + step);
+        float top = 0.0f, inv_total = 1.0f;
         if (!SIGMOID) {
             top = v[0];
 #pragma unroll
             for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
-            top = warp_max(top);
+            top = key_value(__reduce_max_sync(0xffffffffu, order_key(top)));
         }
-        scores<PER, SIGMOID>(v, top, &inv_total);
+        const float total = exponentials<PER, SIGMOID>(v, top);
+        if (!SIGMOID) {
+            inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) v[i] *= inv_total;
+        }
         const float s = score_of<SIGMOID>(l, top, inv_total);
         float d = dw;
         if (p.renormalize) {
-            const float norm = warp_sum(s), inv = norm > 0.0f ? 1.0f / norm : 0.0f;
-            d = (dw - warp_sum(s * inv * dw)) * inv;
+            float norm = s, mean = s * dw;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                norm += __shfl_xor_sync(0xffffffffu, norm, o);
+                mean += __shfl_xor_sync(0xffffffffu, mean, o);
+            }
+            const float inv = norm > 0.0f ? 1.0f / norm : 0.0f;
+            d = (dw - mean * inv) * inv;
         }
-        if (mine < 0) d = 0.0f;
+        float kept = 0.0f;
+        if (mine >= 0) {
+            kept = ds_sm[mine];
+            tag_sm[mine] = static_cast<uint8_t>(lane);
+        }
+        __syncwarp();
+        if (mine >= 0) ds_sm[mine] = kept + d;
+        if (__any_sync(0xffffffffu, mine >= 0 && tag_sm[mine] != lane)) {
+            // a caller's list that names an expert twice: one after the other, in the list's order
+            if (mine >= 0) ds_sm[mine] = kept;
+            __syncwarp();
+            for (int k = 0; k < p.K; ++k) {
+                if (lane == k && mine >= 0) ds_sm[mine] += d;
+                __syncwarp();
+            }
+        }
+        __syncwarp();
         float ds[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = expert_of<VEC>(i, lane);
-            ds[i] = p.d_score_sums && e < p.E ? __ldg(p.d_score_sums + e) : 0.0f;
-        }
-        for (int k = 0; k < p.K; ++k) {
-            const int e = __shfl_sync(0xffffffffu, mine, k);
-            const float dk = __shfl_sync(0xffffffffu, d, k);
-#pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (expert_of<VEC>(i, lane) == e) ds[i] += dk;
-        }
+        for (int i = 0; i < PER; ++i) ds[i] = ds_sm[expert_of<VEC>(i, lane)];
+        __syncwarp();
+        if (mine >= 0) ds_sm[mine] = kept;
+        __syncwarp();
         if (SIGMOID) {
 #pragma unroll
             for (int i = 0; i < PER; ++i) v[i] = ds[i] * v[i] * (1.0f - v[i]);
@@ -312,15 +450,15 @@ __global__ void __launch_bounds__(route_threads(PER)) route_bwd_kernel(const Rou
 }
 
 int route_blocks(int64_t T, int E) {
-    const int warps = route_threads((E + 31) / 32) / 32;
-    const int64_t blocks = (T + warps - 1) / warps, most = 2LL * sm_count();
+    const int per = (E + 31) / 32, warps = route_threads(per) / 32;
+    const int64_t blocks = (T + warps - 1) / warps, most = static_cast<int64_t>(route_blocks_per_sm(per)) * sm_count();
     return static_cast<int>(blocks < most ? blocks : most);
 }
 
 template <int PER, bool BF16, bool VEC, bool SIGMOID>
 int launch_route(const RouteParams& p, bool backward, cudaStream_t stream) {
     const int blocks = route_blocks(p.T, PER * 32);
-    if (backward) route_bwd_kernel<PER, BF16, VEC, SIGMOID><<<blocks, route_threads(PER), 0, stream>>>(p);
+    if (backward) route_bwd_kernel<PER, BF16, VEC, SIGMOID><<<blocks, route_threads(PER), route_threads(PER) * PER * 5, stream>>>(p);
     else route_kernel<PER, BF16, VEC, SIGMOID><<<blocks, route_threads(PER), p.part_count ? 8u * p.E : 0u, stream>>>(p);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
@@ -394,9 +532,8 @@ extern "C" int mokb_route(const void* logits, int bf16, int64_t row_stride, int6
     }
     if (num_tokens > 0) MOKB_TRY(launch_route(p, bf16 != 0, score == MOKB_SCORE_SIGMOID, false, stream));
     if (tokens_per_expert) {
-        route_reduce_kernel<<<(num_experts + 31) / 32, 1024, 0, stream>>>(p.part_count, p.part_sum, blocks, num_experts, tokens_per_expert, score_sums);
-        MOKB_CUDA(cudaGetLastError());
-        note_launch();
+        MOKB_TRY(launch_after(route_reduce_kernel, static_cast<unsigned>((num_experts + 7) / 8), 1024u, 0, stream, static_cast<const int32_t*>(p.part_count),
+                              static_cast<const float*>(p.part_sum), blocks, num_experts, tokens_per_expert, score_sums));
     }
     return MOKB_OK;
 }
