@@ -505,7 +505,7 @@ int mokb_swiglu_bwd(const void* gate, const void* up, const void* d_hidden, void
  * x and hidden quantised to E4M3 along the contraction (weights as in mokb_fwd_mxfp8_args); hidden is rounded to bf16 (or E4M3)
  * between the products, everything else is fp32 until y is rounded.  Four launches; results do not depend on timing.
  *   x, y [num_tokens, hidden] bf16, 16-byte aligned; top_experts [num_tokens, topk] int64; router_weights [num_tokens, topk]
- *   hidden a multiple of 256, intermediate of 128; num_tokens in [0, MOKB_FEW_MAX_TOKENS]
+ *   hidden a multiple of 256, intermediate of 128; num_tokens in [0, MOKB_FEW_MAX_TOKENS], at most 4096 local experts
  *   workspace  mokb_few_tokens_workspace_bytes() bytes of the current device, 256-byte aligned, no initialisation needed, not
  *              shared by calls that may overlap
  *   the shared expert's three weights (bf16) may be NULL together */

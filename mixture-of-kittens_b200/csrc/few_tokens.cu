@@ -42,7 +42,7 @@ constexpr int kSmemLimit = 227 * 1024;
 constexpr int kCtrlBytes = 512 + kLoaderWarps * 512;      // barriers, flags; a row list per loader warp
 // No CTA takes fewer stages than this: below it, what a tile's partial sums cost is more than a stage's load.
 constexpr int kMinStages = 4;
-constexpr int kPlanThreads = 1024, kPlanThreadsSmall = 256, kKept = 4;
+constexpr int kPlanThreads = 1024, kPlanThreadsSmall = 256, kKept = 4, kPlanIds = 8192;
 
 // columns of a unit: two accumulators, double buffered, fill the 512 columns of tensor memory; MXFP8 keeps 32 of them for the scales
 __host__ __device__ constexpr int unit_columns(bool mx) { return mx ? 112 : 128; }
@@ -171,7 +171,8 @@ __device__ __forceinline__ int2 block_scan(int2 v, int2* total) {
 }
 
 // Block 0 lays out the routes; with MXFP8 weights blocks 1.. quantise x, a warp per 1024 values of a row at a time.
-// The order of an expert's tokens is that of the atomics: it decides which column a token gets, not what is computed for it.
+// The order of an expert's tokens is that of the atomics where it has one unit: it decides which column a token gets, not what is computed
+// for it.  Of several units, which one a token is in does (they are cut between CTAs at different places), so those are dealt out in order.
 __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams p) {
     grid_dep_launch();
     const int t0 = threadIdx.x;
@@ -201,7 +202,8 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
         }
         return;
     }
-    extern __shared__ int32_t count[];           // [E] routes, then the experts' first slots
+    extern __shared__ int32_t count[];           // [E] routes, then the experts' first slots; behind them the first kPlanIds routes' experts
+    uint16_t* const ids = reinterpret_cast<uint16_t*>(count + p.E);
     const int NT = p.col_cap, R = p.T * p.K, n_threads = blockDim.x;      // (an expert named twice by a token can have more routes than there are tokens)
     // a thread keeps its first kKept routes in registers between the two passes; further ones leave their number in `pos`
     int expert[kKept], number[kKept];
@@ -211,6 +213,9 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
     };
 #pragma unroll
     for (int i = 0; i < kKept; ++i) expert[i] = t0 + i * n_threads < R ? expert_of(t0 + i * n_threads) : -1;
+#pragma unroll
+    for (int i = 0; i < kKept; ++i)
+        if (t0 + i * n_threads < R) ids[t0 + i * n_threads] = static_cast<uint16_t>(expert[i]);      // (-1: no expert has that number)
     for (int i = t0; i < p.E; i += n_threads) count[i] = 0;
     for (int i = t0; i < 2 * p.sms; i += n_threads) p.w.counters[i] = 0;
     __syncthreads();
@@ -218,9 +223,38 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
     for (int i = 0; i < kKept; ++i) number[i] = expert[i] >= 0 ? atomicAdd(&count[expert[i]], 1) : 0;
     for (int j = t0 + kKept * n_threads; j < R; j += n_threads) {
         const int e = expert_of(j);
+        if (j < kPlanIds) ids[j] = static_cast<uint16_t>(e);
         p.w.pos[j] = e >= 0 ? atomicAdd(&count[e], 1) : -1;
     }
     __syncthreads();
+    bool cut = false;
+    for (int i = t0; i < p.E; i += n_threads) cut = cut || count[i] > NT;
+    if (__syncthreads_or(cut)) {
+        // a warp per such expert goes through the routes in order
+        const int lane = t0 & 31;
+        for (int e = t0 >> 5; e < p.E; e += n_threads >> 5) {
+            if (count[e] <= NT) continue;
+            int before = 0;
+            for (int j0 = lane; j0 - lane < R; j0 += 128) {
+                bool its[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int j = j0 + 32 * i;
+                    its[i] = j < R && (j < kPlanIds ? ids[j] == e : expert_of(j) == e);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned all = __ballot_sync(0xffffffffu, its[i]);
+                    if (its[i]) p.w.pos[j0 + 32 * i] = before + __popc(all & ((1u << lane) - 1u));
+                    before += __popc(all);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kKept; ++i)
+            if (expert[i] >= 0 && count[expert[i]] > NT) number[i] = p.w.pos[t0 + i * n_threads];
+    }
     const int shared_units = p.shared ? (p.T + NT - 1) / NT : 0;
     if (t0 < shared_units) {
         const int lo = t0 * p.T / shared_units, hi = (t0 + 1) * p.T / shared_units;
@@ -469,13 +503,12 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
         }
     } else if (warp >= 2 + kEpilogueWarps) {
         // ------------------------------------------------------------ the tokens' rows
-        if (DOWN) grid_dep_wait();            // hidden
         // Every fourth stage is this warp's as a whole: an arrival per lane and stage costs less than one per lane of four warps.
         const int lw = warp - 2 - kEpilogueWarps, chunk = lane & 7, sub = lane >> 3;      // a lane: 16 bytes of one row of four
         int32_t* const rows = reinterpret_cast<int32_t*>(ctrl + 512 + lw * 512);      // [128]: the row that column n is read from
         int s = 0, turn = 0;
         uint32_t ph = 0;
-        bool ok = true;
+        bool ok = true, waited = !DOWN;
         for (int64_t at = s_begin; ok && at < s_end;) {
             const Segment g = segment_at(st, at, s_end);
             at += g.k1 - g.k0;
@@ -491,6 +524,10 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
                                              : (mx ? p.w.xq : reinterpret_cast<const uint8_t*>(p.x))) + chunk * 16;
             const uint32_t* const scales = DOWN ? reinterpret_cast<const uint32_t*>(p.w.hid_s) : p.w.xs;
             const int kt = (DOWN ? p.I : p.H) / 128;
+            if (!waited) {
+                grid_dep_wait();              // hidden
+                waited = true;
+            }
             for (int k = g.k0; k < g.k1; ++k) {
                 if (turn == lw) {
                     if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT)) { ok = false; break; }
@@ -519,6 +556,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
         const size_t part_stride = static_cast<size_t>(p.col_cap) * 128;      // one accumulator's partial sums
         // slot 1: the tile begins in CTA q (and ends in a later one); slot 0: it began in an earlier one
         auto part_of = [&](int q, int c_lo) { return p.w.part + (static_cast<size_t>(q) * 2 + (q == c_lo ? 1 : 0)) * 2 * part_stride + row; };
+        if (DOWN) grid_dep_wait();      // (no CTA ends before the gate/up kernel has: what follows may overwrite the work area)
         int local = 0, votes = 0;
         for (int64_t at = s_begin; at < s_end; ++local) {
             const Segment g = segment_at(st, at, s_end);
@@ -737,7 +775,7 @@ extern "C" int mokb_few_tokens_fwd(const mokb_few_tokens_args* a, void* stream_)
     TraceScope trace(stream, "few_tokens");
     MOKB_REQUIRE(a != nullptr, "few_tokens: null args");
     MOKB_TRY(check_few_sizes(a->num_tokens, a->hidden, a->intermediate, a->topk));
-    MOKB_REQUIRE(a->num_local_experts >= 1 && a->num_local_experts <= 8192, "few_tokens: num_local_experts must be in [1, 8192]");
+    MOKB_REQUIRE(a->num_local_experts >= 1 && a->num_local_experts <= 4096, "few_tokens: num_local_experts must be in [1, 4096]");
     MOKB_REQUIRE(a->first_expert >= 0, "few_tokens: first_expert must not be negative");
     if (a->num_tokens == 0) return MOKB_OK;
     const bool mx = a->mxfp8 != 0, shared = a->w_shared_gate != nullptr;
@@ -790,7 +828,7 @@ extern "C" int mokb_few_tokens_fwd(const mokb_few_tokens_args* a, void* stream_)
     // few routes: fewer threads to start and to wait for
     const int plan_threads = p.T * p.K <= kPlanThreadsSmall && p.E <= 2 * kPlanThreadsSmall ? kPlanThreadsSmall : kPlanThreads;
     const int pieces = p.T * ((H + 1023) / 1024), quant_blocks = mx ? (pieces + plan_threads / 32 - 1) / (plan_threads / 32) : 0;
-    few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), plan_threads, static_cast<size_t>(p.E) * 4, stream>>>(p);
+    few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), plan_threads, static_cast<size_t>(p.E) * 4 + 2 * (p.T * p.K < kPlanIds ? p.T * p.K : kPlanIds), stream>>>(p);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
     MOKB_TRY(launch_after(few_product_kernel<false>, static_cast<unsigned>(p.sms), kThreads, smem, stream, gu, p));

@@ -565,8 +565,8 @@ def route(logits, bias, topk, sigmoid, renormalize, scale, balance):
         counts = torch.empty(E, dtype=torch.int32, device=dev)
         sums = torch.empty(E, dtype=torch.float32, device=dev)
         scratch = torch.empty(lib.mokb_route_scratch_bytes(T, E), dtype=torch.uint8, device=dev)
-    _ck(lib.mokb_route(_p(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if T > 1 else E, T, E, topk, int(sigmoid),
-                       _p(bias), int(renormalize), scale, _p(top_experts), _p(weights), _p(counts), _p(sums), _p(scratch),
+    _ck(lib.mokb_route(logits.data_ptr(), logits.dtype is torch.bfloat16, logits.stride(0) if T > 1 else E, T, E, topk, sigmoid,
+                       _p(bias), renormalize, scale, top_experts.data_ptr(), weights.data_ptr(), _p(counts), _p(sums), _p(scratch),
                        _stream()))
     return top_experts, weights, counts, sums
 
@@ -574,8 +574,8 @@ def route(logits, bias, topk, sigmoid, renormalize, scale, balance):
 def route_bwd(logits, top_experts, d_router_weights, d_score_sums, sigmoid, renormalize, scale):
     T, E = logits.shape
     d_logits = torch.empty(T, E, dtype=logits.dtype, device=logits.device)
-    _ck(lib.mokb_route_bwd(_p(logits), int(logits.dtype == torch.bfloat16), logits.stride(0) if T > 1 else E, T, E,
-                           top_experts.shape[1], int(sigmoid), int(renormalize), scale, _p(top_experts), _p(d_router_weights),
+    _ck(lib.mokb_route_bwd(logits.data_ptr(), logits.dtype is torch.bfloat16, logits.stride(0) if T > 1 else E, T, E,
+                           top_experts.shape[1], sigmoid, renormalize, scale, _p(top_experts), _p(d_router_weights),
                            _p(d_score_sums), _p(d_logits), _stream()))
     return d_logits
 
@@ -601,7 +601,7 @@ def few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w
 
 def _packed_like(x):
     rows, cols = x.shape
-    return (torch.empty(rows, cols, dtype=torch.int8, device=x.device),
+    return (torch.empty_like(x, dtype=torch.int8),
             torch.empty(rows, (cols + PACK_BLOCK - 1) // PACK_BLOCK, dtype=torch.float32, device=x.device))
 
 
@@ -612,7 +612,7 @@ def pack_rows(x, num_rows=None):
 
 
 def unpack_rows(q, scales, num_rows=None):
-    x = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+    x = torch.empty_like(q, dtype=torch.bfloat16)
     _ck(lib.mokb_unpack_rows(_p(q), _p(scales), _p(x), _p(num_rows), q.shape[0], q.shape[1], _stream()))
     return x
 

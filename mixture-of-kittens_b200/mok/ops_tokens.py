@@ -41,6 +41,11 @@ def _plain(t, dtype, shape, device) -> bool:
     return isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous()
 
 
+def _here(t, dtype) -> bool:
+    """A CUDA tensor of the current device, of `dtype`: the short way past `_check_cuda` (a host microsecond counts in a small call)."""
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.is_cuda and t.get_device() == torch.cuda.current_device()
+
+
 def _check_limit(swiglu_limit) -> None:
     if swiglu_limit is not None and (type(swiglu_limit) not in (int, float) or not swiglu_limit >= 0):
         raise ValueError("swiglu_limit must be None or a non-negative number")
@@ -65,7 +70,8 @@ def _check_logits(logits, topk, score, renormalize, scale) -> tuple[int, int]:
     T, E = logits.shape
     if not topk <= E <= MAX_ROUTE_EXPERTS:
         raise ValueError(f"num_experts must be in [topk, {MAX_ROUTE_EXPERTS}]")
-    _check_cuda("logits", logits, (F32, BF16), contiguous=False)
+    if not (_here(logits, F32) or _here(logits, BF16)):
+        _check_cuda("logits", logits, (F32, BF16), contiguous=False)
     if (E > 1 and logits.stride(1) != 1) or (T > 1 and logits.stride(0) < E):
         raise ValueError("the logits of a token must be contiguous and tokens must not overlap")
     return T, E
@@ -87,7 +93,8 @@ def route(logits, bias, topk, score, renormalize, scale, balance):
     if bias is not None:
         if score != "sigmoid":
             raise ValueError("a bias goes with score 'sigmoid'")
-        _check_cuda("bias", bias, F32, (E,), logits.device)
+        if not _plain(bias, F32, (E,), logits.device):
+            _check_cuda("bias", bias, F32, (E,), logits.device)
     if type(balance) is not bool:
         raise TypeError("balance must be a boolean")
     return _C.route(logits, bias, topk, score == "sigmoid", renormalize, float(scale), balance)
@@ -109,10 +116,12 @@ def route_bwd(
     if topk == 0:
         raise ValueError("top_experts must have shape (num_tokens, topk)")
     T, E = _check_logits(logits, topk, score, renormalize, scale)
-    _check_cuda("top_experts", top_experts, I64, (T, topk), logits.device)
-    _check_cuda("d_router_weights", d_router_weights, F32, (T, topk), logits.device)
-    if d_score_sums is not None:
-        _check_cuda("d_score_sums", d_score_sums, F32, (E,), logits.device)
+    dev = logits.device
+    if not (_plain(top_experts, I64, (T, topk), dev) and _plain(d_router_weights, F32, (T, topk), dev)):
+        _check_cuda("top_experts", top_experts, I64, (T, topk), dev)
+        _check_cuda("d_router_weights", d_router_weights, F32, (T, topk), dev)
+    if d_score_sums is not None and not _plain(d_score_sums, F32, (E,), dev):
+        _check_cuda("d_score_sums", d_score_sums, F32, (E,), dev)
     return _C.route_bwd(logits, top_experts, d_router_weights, d_score_sums, score == "sigmoid", renormalize, float(scale))
 
 
@@ -200,8 +209,10 @@ def _check_packed(name: str, q, scales, device=None) -> tuple[int, int]:
         raise ValueError(f"{name} must have shape (rows, columns)")
     rows, cols = q.shape
     _check_rows(name, rows, cols)
-    _check_cuda(name, q, torch.int8, None, device)
-    _check_cuda(f"{name}'s scales", scales, F32, (rows, -(-cols // PACK_BLOCK)), q.device)
+    shape = (rows, -(-cols // PACK_BLOCK))
+    if not (_here(q, torch.int8) and q.is_contiguous() and (device is None or q.device == device) and _plain(scales, F32, shape, q.device)):
+        _check_cuda(name, q, torch.int8, None, device)
+        _check_cuda(f"{name}'s scales", scales, F32, shape, q.device)
     return rows, cols
 
 
@@ -213,8 +224,10 @@ def pack_rows_op(x: torch.Tensor, num_rows: torch.Tensor | None = None) -> tuple
     if not isinstance(x, torch.Tensor) or x.ndim != 2:
         raise ValueError("x must have shape (rows, columns)")
     _check_rows("x", *x.shape)
-    _check_cuda("x", x, BF16)
-    _check_num_rows(num_rows, x.device)
+    if not (_here(x, BF16) and x.is_contiguous()):
+        _check_cuda("x", x, BF16)
+    if num_rows is not None:
+        _check_num_rows(num_rows, x.device)
     return _C.pack_rows(x, num_rows)
 
 
@@ -222,7 +235,8 @@ def pack_rows_op(x: torch.Tensor, num_rows: torch.Tensor | None = None) -> tuple
 def unpack_rows_op(q: torch.Tensor, scales: torch.Tensor, num_rows: torch.Tensor | None = None) -> torch.Tensor:
     """What `pack_rows` kept, as bf16."""
     _check_packed("q", q, scales)
-    _check_num_rows(num_rows, q.device)
+    if num_rows is not None:
+        _check_num_rows(num_rows, q.device)
     return _C.unpack_rows(q, scales, num_rows)
 
 

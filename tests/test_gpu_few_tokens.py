@@ -130,13 +130,23 @@ def test_no_tokens():
 
 
 @pytest.mark.parametrize("mx", [False, True], ids=["bf16", "mxfp8"])
-def test_two_runs_give_the_same_bits(mx):
+@pytest.mark.parametrize("size", [(37, 1024, 512, 12, 4), (400, 1024, 256, 5, 3)], ids=["one_unit", "cut_experts"])
+def test_two_runs_give_the_same_bits(size, mx):
+    """Also where an expert has more tokens than a unit holds: which of its units a token is in must not change."""
     from mok import functional as F
-    args = make(37, 1024, 512, 12, 4, mx=mx, seed=8)
+    args = make(*size, mx=mx, seed=8)
     x, top, w, sh, routed = args
     first = F.forward_few_tokens(x, top, w, *sh, *routed)
     for _ in range(20):
         assert torch.equal(first, F.forward_few_tokens(x, top, w, *sh, *routed))
+
+
+def test_many_routes():
+    """More routes than the plan's threads keep in registers (over 4096), with and without cut experts."""
+    check(*make(180, 256, 128, 40, 32, seed=13))
+    x, top, w, sh, routed = make(511, 256, 128, 16, 12, seed=14)
+    check(x, top, w, sh, routed)
+    check(x, top, w, [None] * 3, routed, first=3)
 
 
 def test_two_streams_at_once_and_calls_back_to_back():

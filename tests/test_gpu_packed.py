@@ -164,6 +164,23 @@ def test_rows_behind_the_last_stay_as_they_were():
             assert torch.equal(got[:n], want[:n]) and (got[n:] == 9.0).all()
 
 
+def test_offsets_past_32_bits():
+    """More values than 2^31: the last rows of all three."""
+    from mok import ops
+    n, c = 2 ** 20 + 3, 2048
+    tail = rows_of(5, c, seed=31)
+    x = torch.zeros(n, c, dtype=torch.bfloat16, device="cuda")
+    x[-5:] = tail
+    q, s = ops.pack_rows(x)
+    tq, ts = ops.pack_rows(tail)
+    assert torch.equal(q[-5:], tq) and torch.equal(s[-5:], ts) and int(q[:-5].abs().max()) == 0
+    del x
+    assert torch.equal(ops.unpack_rows(q, s)[-5:], ops.unpack_rows(tq, ts))
+    dh = torch.ones(n, c, dtype=torch.bfloat16, device="cuda")
+    got, want = ops.swiglu_bwd_packed(q, s, q, s, dh), ops.swiglu_bwd_packed(tq, ts, tq, ts, dh[:5])
+    assert all(torch.equal(a[-5:], b) for a, b in zip(got, want))
+
+
 def test_no_rows():
     from mok import ops
     q, s = ops.pack_rows(torch.zeros(0, 256, dtype=torch.bfloat16, device="cuda"))

@@ -234,3 +234,41 @@ def test_captured_forward_and_backward():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step()))
+
+
+def test_offsets_past_32_bits():
+    """More logits than 2^31: the last tokens."""
+    from mok import functional as F
+    T, E = 2 ** 25 + 5, 64
+    logits = torch.empty(T, E, dtype=torch.bfloat16, device="cuda")
+    tail = logits_of(9, E, torch.bfloat16, seed=23)
+    logits[:-9] = tail[0]
+    logits[-9:] = tail
+    cfg = F.MoKRouterConfig(topk=3)
+    r = F.route(cfg, logits)
+    want = F.route(cfg, tail)
+    assert torch.equal(r.top_experts[-9:], want.top_experts) and torch.equal(r.router_weights[-9:], want.router_weights)
+    dw = torch.zeros(T, 3, device="cuda")
+    dw[-9:] = torch.randn(9, 3, device="cuda")
+    d = F.route_backward(cfg, logits, r, dw)
+    assert torch.equal(d[-9:], F.route_backward(cfg, tail, want, dw[-9:].contiguous())) and (d[:-9] == 0).all()
+
+
+def test_a_row_whose_order_needs_64_bits():
+    """Biased sums that differ by less than a 32-bit sigmoid's error: the order is that of the exact sums."""
+    from mok import functional as F
+    E, K = 64, 5
+    gen = torch.Generator(device="cuda").manual_seed(24)
+    logits = torch.randn(300, E, generator=gen, device="cuda")
+    s = torch.sigmoid(logits.double())
+    bias = torch.zeros(E, device="cuda")
+    # every row's logits moved so that all scores lie within 1e-6 of 0.7
+    target = 0.7 + (s - 0.5) * 2e-6
+    logits = torch.log(target / (1 - target)).float()
+    check_forward(F.MoKRouterConfig(topk=K, score="sigmoid"), logits, bias)
+    bias = torch.randint(0, 2, (E,), generator=gen, device="cuda").float() * 0.125
+    check_forward(F.MoKRouterConfig(topk=K, score="sigmoid"), logits, bias)
+    # and fp32 logits that agree in all bits but the last ones
+    close = 1.0 + torch.randint(0, 16, (300, E), generator=gen, device="cuda").float() * 2.0 ** -23
+    check_forward(F.MoKRouterConfig(topk=K), close)
+    check_forward(F.MoKRouterConfig(topk=K), -close)

@@ -130,7 +130,7 @@ def test_the_library_checks_sizes_and_addresses():
     refused(few_fwd(w_routed_up=None), b"null weight")
     refused(few_fwd(w_shared_up=4096), b"together")
     refused(few_fwd(mxfp8=1), b"null scales")
-    refused(few_fwd(num_local_experts=8193), b"num_local_experts")
+    refused(few_fwd(num_local_experts=4097), b"num_local_experts")
     assert few_fwd(num_tokens=0) == 0
     assert lib.mokb_few_tokens_workspace_bytes(512, 256, 128, 2, 0) == 0 and lib.mokb_few_tokens_workspace_bytes(1, 256, 128, 2, 0) > 0
 
