@@ -131,7 +131,7 @@ constexpr int index_bits(int per) { return per == 4 ? 7 : per == 8 ? 8 : per == 
 template <int PER, bool CHECK, bool BIASED>
 __device__ __forceinline__ int pick(const uint32_t (&key)[PER], int K, int lane, bool* open) {
     constexpr int B = index_bits(PER);
-    uint32_t b1, b2, mine = 0u, before = 0u;      // b1, b2: this lane's two largest that are not taken
+    uint32_t b1, b2, mine = 0u, last = 0u;        // b1, b2: this lane's two largest that are not taken
     int cached = 2;
     auto look = [&](uint32_t below) {
         b1 = b2 = 0u;
@@ -143,28 +143,30 @@ __device__ __forceinline__ int pick(const uint32_t (&key)[PER], int K, int lane,
         }
     };
     look(0xffffffffu);
-    if (CHECK) *open = false;
     const int rounds = CHECK ? K + 1 : K;
     for (int k = 0; k < rounds; ++k) {
-        const uint32_t top = __reduce_max_sync(0xffffffffu, b1);
-        if (lane == k) mine = top;
-        if (CHECK && k > 0 && (top >> B) > (kClosedKey >> B)) {
-            if (BIASED) {
-                // both keys lost up to 2^(B - 23) of their size to the index
-                const float hi = key_value(before), lo = key_value(top);
-                *open = *open || hi - lo <= 1e-6f + (1e-6f + 2.0f / (1 << (22 - B))) * fmaxf(fabsf(hi), fabsf(lo));
-            } else {
-                *open = *open || ((before ^ top) >> B) == 0u;
-            }
-        }
-        before = top;
-        if (b1 == top) {
+        last = __reduce_max_sync(0xffffffffu, b1);
+        if (lane == k) mine = last;
+        if (b1 == last) {
             b1 = b2;
             if (--cached == 0) {
-                look(top);
+                look(last);
                 cached = 2;
             }
         }
+    }
+    if (CHECK) {
+        uint32_t below = __shfl_down_sync(0xffffffffu, mine, 1);
+        if (lane == K - 1) below = last;
+        bool unsettled;
+        if (BIASED) {
+            // both keys lost up to 2^(B - 23) of their size to the index
+            const float hi = key_value(mine), lo = key_value(below);
+            unsettled = hi - lo <= 1e-6f + (1e-6f + 2.0f / (1 << (22 - B))) * fmaxf(fabsf(hi), fabsf(lo));
+        } else {
+            unsettled = ((mine ^ below) >> B) == 0u;
+        }
+        *open = __any_sync(0xffffffffu, lane < K && (below >> B) > (kClosedKey >> B) && unsettled);
     }
     return ((1 << B) - 1) - static_cast<int>(mine & ((1u << B) - 1u));
 }

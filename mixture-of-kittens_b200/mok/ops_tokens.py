@@ -11,6 +11,7 @@ from . import ops as _ops
 from .ops_mxfp8 import F8, _sc_shape
 
 MAX_FEW_TOKENS = 511
+MAX_FEW_EXPERTS = 4096
 MAX_ROUTE_EXPERTS = 1024
 MAX_ROUTE_TOPK = 32
 PACK_BLOCK = _C.PACK_BLOCK
@@ -157,6 +158,8 @@ def few_tokens_fwd(
     if not isinstance(w_routed_gate, torch.Tensor) or w_routed_gate.ndim != 3 or w_routed_gate.shape[0] <= 0:
         raise ValueError("w_routed_gate must have shape (num_local_experts, intermediate_size, hidden_size)")
     E, I = w_routed_gate.shape[:2]
+    if E > MAX_FEW_EXPERTS:
+        raise ValueError(f"num_local_experts must be at most {MAX_FEW_EXPERTS}")
     if I <= 0 or I % 128 != 0:
         raise ValueError("intermediate_size must be positive and divisible by 128")
     if not isinstance(top_experts, torch.Tensor) or top_experts.ndim != 2 or not 0 < top_experts.shape[1] <= 255:
