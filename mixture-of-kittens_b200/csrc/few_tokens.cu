@@ -255,12 +255,7 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
         for (int i = 0; i < kKept; ++i)
             if (expert[i] >= 0 && count[expert[i]] > NT) number[i] = p.w.pos[t0 + i * n_threads];
     }
-    const int shared_units = p.shared ? (p.T + NT - 1) / NT : 0;
-    if (t0 < shared_units) {
-        const int lo = t0 * p.T / shared_units, hi = (t0 + 1) * p.T / shared_units;
-        p.w.units[t0] = Unit{-1, hi - lo, lo, t0 << 16 | shared_units};
-    }
-    int2 carry = make_int2(0, shared_units);     // slots, units
+    int2 carry = make_int2(0, 0);                // slots, units
     for (int e0 = 0; e0 < p.E; e0 += n_threads) {
         const int e = e0 + t0;
         const int n = e < p.E ? count[e] : 0;
@@ -277,8 +272,13 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
         carry.x += total.x;
         carry.y += total.y;
     }
+    const int shared_units = p.shared ? (p.T + NT - 1) / NT : 0;      // the last ones
+    if (t0 < shared_units) {
+        const int lo = t0 * p.T / shared_units, hi = (t0 + 1) * p.T / shared_units;
+        p.w.units[carry.y + t0] = Unit{-1, hi - lo, lo, t0 << 16 | shared_units};
+    }
     if (t0 == 0) {
-        p.w.header[0] = carry.y;
+        p.w.header[0] = carry.y + shared_units;
         p.w.header[1] = shared_units;
     }
     __syncthreads();
@@ -304,21 +304,21 @@ __global__ void __launch_bounds__(kPlanThreads) few_plan_kernel(const FewParams 
 struct Stream {
     int blocks;                   // tiles of a unit
     int ks_shared, ks_routed;     // stages of a tile
-    int tiles_shared;
-    int64_t shared_stages, total;
+    int tiles_routed;             // they come first
+    int64_t routed_stages, total;
     int ctas;                     // that take part
     __device__ Stream(const FewParams& p, int units, int shared_units, bool down) {
         const int contraction = down ? p.I : p.H;
         blocks = down ? p.H / 256 : p.I / 128;
         ks_shared = contraction / 64;
         ks_routed = p.mx ? contraction / 128 : contraction / 64;
-        tiles_shared = shared_units * blocks;
-        shared_stages = static_cast<int64_t>(tiles_shared) * ks_shared;
-        total = shared_stages + static_cast<int64_t>(units - shared_units) * blocks * ks_routed;
+        tiles_routed = (units - shared_units) * blocks;
+        routed_stages = static_cast<int64_t>(tiles_routed) * ks_routed;
+        total = routed_stages + static_cast<int64_t>(shared_units) * blocks * ks_shared;
         const int64_t most = total / kMinStages;
         ctas = most < 1 ? 1 : most < p.sms ? static_cast<int>(most) : p.sms;
     }
-    __device__ int64_t begin(int c) const { return c * total / ctas; }
+    __device__ int64_t begin(int64_t c) const { return c * total / ctas; }
     __device__ int owner(int64_t stage) const { return static_cast<int>(((stage + 1) * ctas - 1) / total); }
 };
 struct Segment {
@@ -327,15 +327,15 @@ struct Segment {
 };
 __device__ __forceinline__ Segment segment_at(const Stream& st, int64_t s, int64_t end) {
     Segment g;
-    if (s < st.shared_stages) {
-        g.ks = st.ks_shared;
+    if (s < st.routed_stages) {
+        g.ks = st.ks_routed;
         g.tile = static_cast<int>(s / g.ks);
         g.first = static_cast<int64_t>(g.tile) * g.ks;
     } else {
-        g.ks = st.ks_routed;
-        const int64_t r = (s - st.shared_stages) / g.ks;
-        g.tile = st.tiles_shared + static_cast<int>(r);
-        g.first = st.shared_stages + r * g.ks;
+        g.ks = st.ks_shared;
+        const int64_t r = (s - st.routed_stages) / g.ks;
+        g.tile = st.tiles_routed + static_cast<int>(r);
+        g.first = st.routed_stages + r * g.ks;
     }
     g.k0 = static_cast<int>(s - g.first);
     const int64_t left = end - g.first;
@@ -828,7 +828,8 @@ extern "C" int mokb_few_tokens_fwd(const mokb_few_tokens_args* a, void* stream_)
     // few routes: fewer threads to start and to wait for
     const int plan_threads = p.T * p.K <= kPlanThreadsSmall && p.E <= 2 * kPlanThreadsSmall ? kPlanThreadsSmall : kPlanThreads;
     const int pieces = p.T * ((H + 1023) / 1024), quant_blocks = mx ? (pieces + plan_threads / 32 - 1) / (plan_threads / 32) : 0;
-    few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), plan_threads, static_cast<size_t>(p.E) * 4 + 2 * (p.T * p.K < kPlanIds ? p.T * p.K : kPlanIds), stream>>>(p);
+    few_plan_kernel<<<1 + (quant_blocks < p.sms ? quant_blocks : p.sms), plan_threads,
+                      static_cast<size_t>(p.E) * 4 + 2 * (p.T * p.K < kPlanIds ? p.T * p.K : kPlanIds), stream>>>(p);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
     MOKB_TRY(launch_after(few_product_kernel<false>, static_cast<unsigned>(p.sms), kThreads, smem, stream, gu, p));
