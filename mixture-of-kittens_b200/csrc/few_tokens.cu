@@ -18,8 +18,18 @@
 // Work is cut by stages of the contraction, not by tiles: the stages of all tiles are numbered through and every CTA takes an equal,
 // contiguous range (7 experts of 1408 x 5120 are 77 gate/up tiles on 148 SMs).  A tile that falls to several CTAs is summed by the one
 // that finishes last, in the order of the contraction, from fp32 partial sums in global memory: nobody waits, so calls on several
-// streams cannot block each other, and the result does not depend on who was last.  The same way the down projection's results of a
-// token (fp32, one row per route) are summed over its experts, in the order k = 0, 1, .., by the warp that counts the last of them.
+// streams cannot block each other, and the result does not depend on who was last.  (Summing the routes of a token the same way, by
+// whoever counts its last one, put a fence and four dependent round trips to a busy memory into every tile: down 260 us instead of 135
+// for 24 tokens through 64 experts of 5120 x 1408.  So that is a launch of its own.)
+//
+// Graph replays back to back, weights from memory (6546 GB/s: a plain copy's rate here): one token through 8 of 32 experts of 7168 x 2048
+// and the shared one 138 us (5.7 TB/s), 24 tokens through 64 of 5120 x 1408 389 us (6.5 TB/s), 48 tokens on one of two ranks' 64 experts of
+// 4096 x 1536 in MXFP8 196 us (5.9 TB/s), 200 tokens through all of the first 528 us (5.5 TB/s), two tokens of the smallest layer (8 of
+// 1024 x 512) 24 us.  One token: 5 us until the first weights arrive (plan, header, unit, memory), 3 us between the products (the last
+// tiles' sums), the SMs end 8 us apart, 5 us for the sum and its launch.  Two tokens of the small layer are a chain of such latencies.
+// What bounds a stage where memory does not: eight MMAs take about 45 clocks each whatever N is, of the 1300 that its 32 KB take to arrive.
+// Three stages in the ring instead of six cost 4 %; units of 64 columns instead of 128 nothing up to 200 tokens, 45 % at 511 (their experts'
+// weights are then read twice).
 //
 //   warp 0     TMA producer: weights (two 128-row boxes of 128 bytes per stage) and, MXFP8, their scale tiles
 //   warp 1     MMA issuer
@@ -40,8 +50,10 @@ constexpr int SF_BYTES = 3 * 512;               // MXFP8: the scale tiles of bot
 constexpr int kMaxStages = 8;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kCtrlBytes = 512 + kLoaderWarps * 512;      // barriers, flags; a row list per loader warp
-// No CTA takes fewer stages than this: below it, what a tile's partial sums cost is more than a stage's load.
+// No CTA takes fewer stages than this: below it, what a tile's partial sums cost is more than a stage's load.  (Two tokens, 8 experts of
+// 1024 x 512: 24.3 us; with 2 stages 28, with 6 25.1, with 8 23.6, with 16 28.2.)
 constexpr int kMinStages = 4;
+// plan: threads, fewer for few routes; routes that a thread keeps in registers; routes whose experts are kept in shared memory
 constexpr int kPlanThreads = 1024, kPlanThreadsSmall = 256, kKept = 4, kPlanIds = 8192;
 
 // columns of a unit: two accumulators, double buffered, fill the 512 columns of tensor memory; MXFP8 keeps 32 of them for the scales
@@ -503,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
         }
     } else if (warp >= 2 + kEpilogueWarps) {
         // ------------------------------------------------------------ the tokens' rows
-        // Every fourth stage is this warp's as a whole: an arrival per lane and stage costs less than one per lane of four warps.
+        // Every fourth stage is this warp's as a whole.
         const int lw = warp - 2 - kEpilogueWarps, chunk = lane & 7, sub = lane >> 3;      // a lane: 16 bytes of one row of four
         int32_t* const rows = reinterpret_cast<int32_t*>(ctrl + 512 + lw * 512);      // [128]: the row that column n is read from
         int s = 0, turn = 0;

@@ -61,7 +61,8 @@ __device__ __forceinline__ uint4 pack_16(const uint32_t (&w)[8], float* scale) {
 // byte j of a word as a signed number
 __device__ __forceinline__ float signed_byte(uint32_t w, int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); }
 
-// 135168 x 2048: 147 us, 5.7 TB/s (two groups of four blocks in flight per warp: 157 us); 135168 x 7168: 498 us, 5.9 TB/s.
+// 135168 x 2048: 143 us, 5.9 TB/s (16 blocks per SM instead of 32: 147, a block for every 64 scales: 159; two groups of four scales in
+// flight per warp: 157); 135168 x 7168: 490 us, 6.0 TB/s.
 // A warp takes four blocks at a time.  `per_row` blocks of a row, the last one shorter where 128 does not divide cols.
 __global__ void __launch_bounds__(256) pack_kernel(const __nv_bfloat16* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scales,
                                                    const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row) {
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const __nv_bfloat16* __restri
     }
 }
 
+// 135168 x 2048: 130 us, 6.5 TB/s, every thread one unit (16 blocks per SM that go on: 145); 135168 x 7168: 435 us, 6.7 TB/s.
 __global__ void __launch_bounds__(256) unpack_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales, __nv_bfloat16* __restrict__ x,
                                                      const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row) {
     const int64_t items = live_rows(num_rows, rows_cap) * (cols / 16), stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -115,7 +117,7 @@ __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.N
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
 // One warp per row; the row's sum of d_hidden * hidden, divided by its router weight, in a fixed order.
-// 135168 x 2048: 461 us, 6.05 TB/s; 25088 x 1408: 73 us.  The IEEE quotient is not what bounds it: with the approximate one the compiler
+// 135168 x 2048: 457 us, 6.1 TB/s; 25088 x 1408: 73 us.  The IEEE quotient is not what bounds it: with the approximate one the compiler
 // takes 101 registers (577 us; held to 64: 534), and eight values per lane at a time (more warps, smaller accesses) take 526 to 596 us.
 __global__ void __launch_bounds__(256) swiglu_bwd_packed_kernel(
     const int8_t* __restrict__ gate_q, const float* __restrict__ gate_sc, const int8_t* __restrict__ up_q, const float* __restrict__ up_sc,
@@ -196,7 +198,7 @@ extern "C" int mokb_pack_rows(const void* x, void* q, float* scales, const int32
     MOKB_REQUIRE(x && q && scales, "pack_rows: null pointer");
     MOKB_REQUIRE(aligned(x, 32) && aligned(q, 16), "pack_rows: x must be 32-byte and q 16-byte aligned");
     const int per_row = static_cast<int>((cols + kBlock - 1) / kBlock);
-    pack_kernel<<<blocks_for(rows * per_row * 8, 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    pack_kernel<<<blocks_for(rows * per_row * 8, 32), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const __nv_bfloat16*>(x), static_cast<int8_t*>(q), scales, num_rows, rows, static_cast<int>(cols), per_row);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
@@ -209,7 +211,7 @@ extern "C" int mokb_unpack_rows(const void* q, const float* scales, void* x, con
     if (rows == 0) return MOKB_OK;
     MOKB_REQUIRE(x && q && scales, "unpack_rows: null pointer");
     MOKB_REQUIRE(aligned(x, 32) && aligned(q, 16), "unpack_rows: x must be 32-byte and q 16-byte aligned");
-    unpack_kernel<<<blocks_for(rows * (cols / 16), 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    unpack_kernel<<<blocks_for(rows * (cols / 16), 4096), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const int8_t*>(q), scales, static_cast<__nv_bfloat16*>(x), num_rows, rows, static_cast<int>(cols),
         static_cast<int>((cols + kBlock - 1) / kBlock));
     MOKB_CUDA(cudaGetLastError());
@@ -227,7 +229,7 @@ extern "C" int mokb_swiglu_bwd_packed(const void* gate_q, const float* gate_scal
     MOKB_REQUIRE(gate_q && gate_scales && up_q && up_scales && d_hidden && d_gate && d_up && hidden, "swiglu_bwd_packed: null pointer");
     MOKB_REQUIRE(aligned(gate_q, 16) && aligned(up_q, 16) && aligned(d_hidden, 32) && aligned(d_gate, 32) && aligned(d_up, 32) && aligned(hidden, 32),
                  "swiglu_bwd_packed: packed tensors must be 16-byte and bf16 tensors 32-byte aligned");
-    swiglu_bwd_packed_kernel<<<blocks_for(rows * 32, 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    swiglu_bwd_packed_kernel<<<blocks_for(rows * 32, 32), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const int8_t*>(gate_q), gate_scales, static_cast<const int8_t*>(up_q), up_scales, static_cast<const __nv_bfloat16*>(d_hidden),
         static_cast<__nv_bfloat16*>(d_gate), static_cast<__nv_bfloat16*>(d_up), static_cast<__nv_bfloat16*>(hidden), row_scale, row_grad_out,
         num_rows, rows, static_cast<int>(cols), static_cast<int>((cols + kBlock - 1) / kBlock), has_limit, limit);

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -105,6 +106,10 @@ class FewTokensArgs(ctypes.Structure):
                                "w_routed_down_sc", "y", "workspace", "status")])
 
 
+# the same layout, filled in one go (the fields of a ctypes structure take 0.1 us of host time each)
+_pack_few = struct.Struct("@8if15P").pack
+
+
 class PackedContext(ctypes.Structure):
     _fields_ = [(f"{n}_{part}", c_vp) for n in ("x_routed", "gate_routed", "up_routed", "gate_shared", "up_shared")
                 for part in ("q", "scales")]
@@ -152,6 +157,8 @@ _sig("mokb_swiglu_bwd", c_int, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c
 _sig("mokb_few_tokens_args_size", c_sz)
 _sig("mokb_few_tokens_workspace_bytes", c_sz, c_int, c_int, c_int, c_int, c_int)
 _sig("mokb_few_tokens_fwd", c_int, ctypes.POINTER(FewTokensArgs), c_vp)
+_few_tokens_fwd_packed = lib["mokb_few_tokens_fwd"]              # the same function, its argument as bytes
+_few_tokens_fwd_packed.restype, _few_tokens_fwd_packed.argtypes = c_int, [ctypes.c_char_p, c_vp]
 _sig("mokb_route_scratch_bytes", c_sz, c_i64, c_int)
 _sig("mokb_route", c_int, c_vp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_vp, c_int, c_f32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp)
 _sig("mokb_route_bwd", c_int, c_vp, c_int, c_i64, c_i64, c_int, c_int, c_int, c_int, c_f32, c_vp, c_vp, c_vp, c_vp, c_vp)
@@ -199,7 +206,7 @@ def _check_struct_layout():
     mine = (ctypes.sizeof(FwdArgs), ctypes.sizeof(BwdArgs), ctypes.sizeof(GemmArgs))
     if tuple(sizes) != mine:
         raise ImportError(f"struct layout mismatch between _C.py {mine} and libmok_b200.so {tuple(sizes)}")
-    if ctypes.sizeof(FewTokensArgs) != lib.mokb_few_tokens_args_size():
+    if not ctypes.sizeof(FewTokensArgs) == struct.calcsize("@8if15P") == lib.mokb_few_tokens_args_size():
         raise ImportError("struct layout mismatch between _C.py and libmok_b200.so: FewTokensArgs")
 
 
@@ -585,17 +592,17 @@ def few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w
     """`scales`: None, or the packed scales of the three routed weights (MXFP8).  The work area is a tensor of this call:
     calls on several streams, or captured in several graphs, do not share it."""
     T, H = x.shape
-    E, I = w_routed_gate.shape[:2]
+    E, I, _ = w_routed_gate.shape
     K = top_experts.shape[1]
-    mx = int(scales is not None)
+    mx = scales is not None
+    sg, su, sd = (0, 0, 0) if w_shared_gate is None else (w_shared_gate.data_ptr(), w_shared_up.data_ptr(), w_shared_down.data_ptr())
+    gs, us, ds = (scales[0].data_ptr(), scales[1].data_ptr(), scales[2].data_ptr()) if mx else (0, 0, 0)
     y = torch.empty_like(x)
     work = torch.empty(lib.mokb_few_tokens_workspace_bytes(T, H, I, K, mx), dtype=torch.uint8, device=x.device)
-    a = FewTokensArgs(T, H, I, E, K, first_expert, mx, 0 if swiglu_limit is None else 1,
-                      0.0 if swiglu_limit is None else float(swiglu_limit), _p(x), _p(top_experts), _p(router_weights),
-                      _p(w_shared_gate), _p(w_shared_up), _p(w_shared_down), _p(w_routed_gate), _p(w_routed_up),
-                      _p(w_routed_down), *((None,) * 3 if scales is None else map(_p, scales)), _p(y), _p(work),
-                      _p(status_tensor(x.device)))
-    _ck(lib.mokb_few_tokens_fwd(ctypes.byref(a), _stream()))
+    args = _pack_few(T, H, I, E, K, first_expert, mx, swiglu_limit is not None, swiglu_limit or 0.0, x.data_ptr(), top_experts.data_ptr(),
+                     router_weights.data_ptr(), sg, su, sd, w_routed_gate.data_ptr(), w_routed_up.data_ptr(), w_routed_down.data_ptr(),
+                     gs, us, ds, y.data_ptr(), work.data_ptr(), status_tensor(x.device).data_ptr())
+    _ck(_few_tokens_fwd_packed(args, _stream()))
     return y
 
 

@@ -157,7 +157,7 @@ def few_tokens_fwd(
         raise ValueError("hidden_size must be positive and divisible by 256")
     if not isinstance(w_routed_gate, torch.Tensor) or w_routed_gate.ndim != 3 or w_routed_gate.shape[0] <= 0:
         raise ValueError("w_routed_gate must have shape (num_local_experts, intermediate_size, hidden_size)")
-    E, I = w_routed_gate.shape[:2]
+    E, I, _ = w_routed_gate.shape
     if E > MAX_FEW_EXPERTS:
         raise ValueError(f"num_local_experts must be at most {MAX_FEW_EXPERTS}")
     if I <= 0 or I % 128 != 0:
@@ -169,31 +169,35 @@ def few_tokens_fwd(
         raise ValueError("first_expert must be a non-negative integer")
     if swiglu_limit is not None:
         _check_limit(swiglu_limit)
-    _check_cuda("x", x, BF16)
+    if not (_here(x, BF16) and x.is_contiguous()):
+        _check_cuda("x", x, BF16)
     dev = x.device
-    scales = (w_routed_gate_sc, w_routed_up_sc, w_routed_down_sc)
-    shared = (w_shared_gate, w_shared_up, w_shared_down)
-    mx = scales[0] is not None
-    table = [("top_experts", top_experts, I64, (T, K)), ("router_weights", router_weights, F32, (T, K)),
-             ("w_routed_gate", w_routed_gate, F8 if mx else BF16, (E, I, H)), ("w_routed_up", w_routed_up, F8 if mx else BF16, (E, I, H)),
-             ("w_routed_down", w_routed_down, F8 if mx else BF16, (E, H, I))]
-    if mx or scales[1] is not None or scales[2] is not None:
-        if any(s is None for s in scales):
-            raise ValueError("the scales of the routed weights go together")
-        table += [(f"{name}_sc", sc, torch.uint8, _sc_shape(E * rows, cols)) for name, sc, rows, cols in
-                  zip(("w_routed_gate", "w_routed_up", "w_routed_down"), scales, (I, I, H), (H, H, I))]
-    if shared[0] is not None or shared[1] is not None or shared[2] is not None:
-        if any(w is None for w in shared):
-            raise ValueError("the shared expert's weights go together")
-        table += [("w_shared_gate", w_shared_gate, BF16, (I, H)), ("w_shared_up", w_shared_up, BF16, (I, H)),
-                  ("w_shared_down", w_shared_down, BF16, (H, I))]
-    for name, t, dtype, shape in table:
-        if not _plain(t, dtype, shape, dev):
+    mx = w_routed_gate_sc is not None
+    if (w_routed_up_sc is not None) != mx or (w_routed_down_sc is not None) != mx:
+        raise ValueError("the scales of the routed weights go together")
+    shared = w_shared_gate is not None
+    if (w_shared_up is not None) != shared or (w_shared_down is not None) != shared:
+        raise ValueError("the shared expert's weights go together")
+    wt = F8 if mx else BF16
+    routed, routed_down = (E, I, H), (E, H, I)
+    if not (_plain(top_experts, I64, (T, K), dev) and _plain(router_weights, F32, (T, K), dev) and _plain(w_routed_gate, wt, routed, dev)
+            and _plain(w_routed_up, wt, routed, dev) and _plain(w_routed_down, wt, routed_down, dev)):
+        for name, t, dtype, shape in (("top_experts", top_experts, I64, (T, K)), ("router_weights", router_weights, F32, (T, K)),
+                                      ("w_routed_gate", w_routed_gate, wt, routed), ("w_routed_up", w_routed_up, wt, routed),
+                                      ("w_routed_down", w_routed_down, wt, routed_down)):
             _check_cuda(name, t, dtype, shape, dev)
+    if mx:
+        for name, t, rows, cols in (("w_routed_gate_sc", w_routed_gate_sc, I, H), ("w_routed_up_sc", w_routed_up_sc, I, H),
+                                    ("w_routed_down_sc", w_routed_down_sc, H, I)):
+            if not _plain(t, torch.uint8, _sc_shape(E * rows, cols), dev):
+                _check_cuda(name, t, torch.uint8, _sc_shape(E * rows, cols), dev)
+    if shared and not (_plain(w_shared_gate, BF16, (I, H), dev) and _plain(w_shared_up, BF16, (I, H), dev) and _plain(w_shared_down, BF16, (H, I), dev)):
+        for name, t, shape in (("w_shared_gate", w_shared_gate, (I, H)), ("w_shared_up", w_shared_up, (I, H)), ("w_shared_down", w_shared_down, (H, I))):
+            _check_cuda(name, t, BF16, shape, dev)
     if T == 0:
         return torch.empty_like(x)
-    return _C.few_tokens_fwd(x, top_experts, router_weights, *shared, w_routed_gate, w_routed_up, w_routed_down,
-                             scales if mx else None, first_expert, swiglu_limit)
+    return _C.few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w_shared_down, w_routed_gate, w_routed_up,
+                             w_routed_down, (w_routed_gate_sc, w_routed_up_sc, w_routed_down_sc) if mx else None, first_expert, swiglu_limit)
 
 
 # ---------------------------------------------------------------------------------------------------------------- 8-bit activations
