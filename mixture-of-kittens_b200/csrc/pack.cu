@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kBlock = 128;
 constexpr float kSmallest = 7.70371977754894e-34f;        // 2^-110
+constexpr float kRound = 12582912.0f;
 
 __device__ __forceinline__ int64_t live_rows(const int32_t* num_rows, int64_t cap) {
     if (!num_rows) return cap;
@@ -46,23 +47,24 @@ __device__ __forceinline__ uint4 pack_16(const uint32_t (&w)[8], float* scale) {
     uint32_t o[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        uint32_t word = 0u;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t pair = w[2 * i + j];
-            const int a = bad ? 0 : __float2int_rn(bf16_lo(pair) * inv), b = bad ? 0 : __float2int_rn(bf16_hi(pair) * inv);
-            word |= ((static_cast<uint32_t>(a) & 0xffu) | (static_cast<uint32_t>(b) & 0xffu) << 8) << (16 * j);
-        }
-        o[i] = word;
+        // 1.5 * 2^23 more: the sum's last place is 1, so that it is rounded to a whole number, whose low byte is the float's
+        const uint32_t a = __float_as_uint(fmaf(bf16_lo(w[2 * i]), inv, kRound)), b = __float_as_uint(fmaf(bf16_hi(w[2 * i]), inv, kRound));
+        const uint32_t c = __float_as_uint(fmaf(bf16_lo(w[2 * i + 1]), inv, kRound)), d = __float_as_uint(fmaf(bf16_hi(w[2 * i + 1]), inv, kRound));
+        o[i] = bad ? 0u : __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
     }
     return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// byte j of a word as a signed number
-__device__ __forceinline__ float signed_byte(uint32_t w, int j) { return static_cast<float>(static_cast<int8_t>(w >> (8 * j))); }
+// The four signed bytes of a word as numbers, through the mantissa of 2^23 + byte + 128 (exact; a conversion instruction per byte is a
+// quarter-rate one, of which the exponential and the quotient have enough).
+__device__ __forceinline__ void signed_bytes(uint32_t w, float (&f)[4]) {
+    w ^= 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7540u + j)) - 8388736.0f;
+}
 
-// 135168 x 2048: 143 us, 5.9 TB/s (16 blocks per SM instead of 32: 147, a block for every 64 scales: 159; two groups of four scales in
-// flight per warp: 157); 135168 x 7168: 490 us, 6.0 TB/s.
+// 135168 x 2048: 130 us, 6.5 TB/s (with a float-to-integer conversion per value: 143); 135168 x 7168: 449 us, 6.5 TB/s.  Before that, 16 blocks per
+// SM instead of 32 took 147 for 143, a block for every 64 scales 159, two groups of four scales in flight per warp 157.
 // A warp takes four blocks at a time.  `per_row` blocks of a row, the last one shorter where 128 does not divide cols.
 __global__ void __launch_bounds__(256) pack_kernel(const __nv_bfloat16* __restrict__ x, int8_t* __restrict__ q, float* __restrict__ scales,
                                                    const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row) {
@@ -88,7 +90,8 @@ __global__ void __launch_bounds__(256) pack_kernel(const __nv_bfloat16* __restri
     }
 }
 
-// 135168 x 2048: 130 us, 6.5 TB/s, every thread one unit (16 blocks per SM that go on: 145); 135168 x 7168: 435 us, 6.7 TB/s.
+// 135168 x 2048: 125 us, 6.7 TB/s, every thread one unit (with a conversion per byte 130, and 145 where 16 blocks per SM go on);
+// 135168 x 7168: 432 us, 6.8 TB/s.
 __global__ void __launch_bounds__(256) unpack_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales, __nv_bfloat16* __restrict__ x,
                                                      const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row) {
     const int64_t items = live_rows(num_rows, rows_cap) * (cols / 16), stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
@@ -106,8 +109,10 @@ __global__ void __launch_bounds__(256) unpack_kernel(const int8_t* __restrict__ 
         uint32_t o[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            o[2 * j] = pack2(signed_byte(w[j], 0) * s, signed_byte(w[j], 1) * s);
-            o[2 * j + 1] = pack2(signed_byte(w[j], 2) * s, signed_byte(w[j], 3) * s);
+            float f[4];
+            signed_bytes(w[j], f);
+            o[2 * j] = pack2(f[0] * s, f[1] * s);
+            o[2 * j + 1] = pack2(f[2] * s, f[3] * s);
         }
         st_global_32B(x + i * 16, o);
     }
@@ -116,60 +121,81 @@ __global__ void __launch_bounds__(256) unpack_kernel(const int8_t* __restrict__ 
 __device__ __forceinline__ float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 
-// One warp per row; the row's sum of d_hidden * hidden, divided by its router weight, in a fixed order.
-// 135168 x 2048: 457 us, 6.1 TB/s; 25088 x 1408: 73 us.  The IEEE quotient is not what bounds it: with the approximate one the compiler
-// takes 101 registers (577 us; held to 64: 534), and eight values per lane at a time (more warps, smaller accesses) take 526 to 596 us.
-__global__ void __launch_bounds__(256) swiglu_bwd_packed_kernel(
+// A block takes up to eight consecutive rows, its threads their units in order, so that no lane idles behind a row's end and what is open
+// in memory at a time is whole rows; the rows' sums of d_hidden * hidden go through shared memory, one number per unit, and are added up
+// in a fixed order.  135168 x 2048 back to back: 450 us, 6.2 TB/s (a warp per row with a conversion per byte: 506; a warp per row: 468; two rows
+// to a block: 509, sixteen: 450); one launch at 25088 x 1408 with a limit: 68 us (73, 77, 94, 70).  Held to 48 registers, a few of which
+// spill: with 64, 75 and 480 to 500 us, with 40, 80 and 482.
+// Back to back it is the board's power that bounds it (1 kW, 1.6 of 1.97 GHz), so instructions count: the sigmoid's quotient is the
+// approximate one, 2 steps of fp32 off where bf16 keeps 2^15 of them (IEEE: 500).
+constexpr int kRowsPerBlock = 8, kUnitsPerBlock = 8192;
+template <bool LIMIT>
+__global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
     const int8_t* __restrict__ gate_q, const float* __restrict__ gate_sc, const int8_t* __restrict__ up_q, const float* __restrict__ up_sc,
     const __nv_bfloat16* __restrict__ d_hidden, __nv_bfloat16* __restrict__ d_gate, __nv_bfloat16* __restrict__ d_up,
     __nv_bfloat16* __restrict__ hidden, const float* __restrict__ row_scale, float* __restrict__ row_grad,
-    const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row, int has_limit, float limit) {
-    const int64_t rows = live_rows(num_rows, rows_cap), warps = static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5);
-    const int lane = threadIdx.x & 31, units = cols / 16;
-    const float lim = has_limit ? limit : __int_as_float(0x7f800000);
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5); row < rows; row += warps) {
-        float sum = 0.0f;
-        float inv_w = 1.0f;
-        if (row_grad && row_scale) {
-            const float w = row_scale[row];
-            inv_w = w > 0.0f ? 1.0f / w : 0.0f;
-        }
-        for (int u = lane; u < units; u += 32) {
-            const int64_t at = row * cols + u * 16, block = row * per_row + (u >> 3);
+    const int32_t* __restrict__ num_rows, int64_t rows_cap, int cols, int per_row, int rows_per_block, float limit) {
+    extern __shared__ float unit_sum[];
+    const int64_t rows = live_rows(num_rows, rows_cap);
+    const int units = cols / 16;
+    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * rows_per_block; row0 < rows; row0 += static_cast<int64_t>(gridDim.x) * rows_per_block) {
+        const int n = static_cast<int>(rows - row0 < rows_per_block ? rows - row0 : rows_per_block), items = n * units;
+        for (int i = threadIdx.x; i < items; i += 256) {
+            const int r = i / units, u = i - r * units;
+            const int64_t at = row0 * cols + static_cast<int64_t>(i) * 16, block = (row0 + r) * per_row + (u >> 3);
             const uint4 gv = ld_once(gate_q + at), uv = ld_once(up_q + at);
             uint32_t dh[8];
             ld_global_32B(d_hidden + at, dh);
             const float gs = __ldg(gate_sc + block), us = __ldg(up_sc + block);
             const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
             uint32_t og[8], ou[8], oh[8];
+            float sum = 0.0f;
+            float inv_w = 1.0f;
+            if (row_grad && row_scale) {
+                const float w = __ldg(row_scale + row0 + r);
+                inv_w = w > 0.0f ? 1.0f / w : 0.0f;
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float dg[2], du[2], h[2];
+            for (int j = 0; j < 4; ++j) {
+                float g4[4], u4[4], dg[4], du[4], h[4];
+                signed_bytes(gw[j], g4);
+                signed_bytes(uw[j], u4);
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const int byte = 2 * (j & 1) + b;
-                    const float g0 = signed_byte(gw[j >> 1], byte) * gs, u0 = signed_byte(uw[j >> 1], byte) * us;
-                    const float d = b ? bf16_hi(dh[j]) : bf16_lo(dh[j]);
-                    const float g = min_nan(g0, lim), up = min_nan(max_nan(u0, -lim), lim);
-                    const float sig = 1.0f / (1.0f + __expf(-g));
+                for (int b = 0; b < 4; ++b) {
+                    const float g0 = g4[b] * gs, u0 = u4[b] * us;
+                    const float d = b & 1 ? bf16_hi(dh[2 * j + (b >> 1)]) : bf16_lo(dh[2 * j + (b >> 1)]);
+                    const float g = LIMIT ? min_nan(g0, limit) : g0, up = LIMIT ? min_nan(max_nan(u0, -limit), limit) : u0;
+                    const float sig = __fdividef(0.25f, fmaf(0.25f, __expf(-g), 0.25f));
                     const float silu = g * sig;
                     h[b] = silu * up;
-                    dg[b] = g0 > lim ? 0.0f : ((1.0f - silu) * sig + silu) * up * d;
-                    du[b] = u0 > lim || u0 < -lim ? 0.0f : silu * d;
+                    dg[b] = ((1.0f - silu) * sig + silu) * up * d;
+                    du[b] = silu * d;
+                    if (LIMIT && g0 > limit) dg[b] = 0.0f;
+                    if (LIMIT && (u0 > limit || u0 < -limit)) du[b] = 0.0f;
                     sum += d * inv_w * h[b];
                 }
-                og[j] = pack2(dg[0], dg[1]);
-                ou[j] = pack2(du[0], du[1]);
-                oh[j] = pack2(h[0], h[1]);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    og[2 * j + b] = pack2(dg[2 * b], dg[2 * b + 1]);
+                    ou[2 * j + b] = pack2(du[2 * b], du[2 * b + 1]);
+                    oh[2 * j + b] = pack2(h[2 * b], h[2 * b + 1]);
+                }
             }
             st_global_32B(d_gate + at, og);
             st_global_32B(d_up + at, ou);
             st_global_32B(hidden + at, oh);
+            if (row_grad) unit_sum[i] = sum;
         }
         if (row_grad) {
+            __syncthreads();
+            for (int r = threadIdx.x >> 5; r < n; r += 8) {
+                float sum = 0.0f;
+                for (int u = threadIdx.x & 31; u < units; u += 32) sum += unit_sum[r * units + u];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            if (lane == 0) row_grad[row] = sum;
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if ((threadIdx.x & 31) == 0) row_grad[row0 + r] = sum;
+            }
+            __syncthreads();
         }
     }
 }
@@ -225,14 +251,18 @@ extern "C" int mokb_swiglu_bwd_packed(const void* gate_q, const float* gate_scal
                                       void* stream) {
     TraceScope trace(static_cast<cudaStream_t>(stream), "swiglu_bwd_packed");
     CHECK_PACK("swiglu_bwd_packed");
+    MOKB_REQUIRE(cols <= 16 * kUnitsPerBlock, "swiglu_bwd_packed: at most 131072 columns");
     if (rows == 0) return MOKB_OK;
     MOKB_REQUIRE(gate_q && gate_scales && up_q && up_scales && d_hidden && d_gate && d_up && hidden, "swiglu_bwd_packed: null pointer");
     MOKB_REQUIRE(aligned(gate_q, 16) && aligned(up_q, 16) && aligned(d_hidden, 32) && aligned(d_gate, 32) && aligned(d_up, 32) && aligned(hidden, 32),
                  "swiglu_bwd_packed: packed tensors must be 16-byte and bf16 tensors 32-byte aligned");
-    swiglu_bwd_packed_kernel<<<blocks_for(rows * 32, 32), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+    auto* const kernel = has_limit ? swiglu_bwd_packed_kernel<true> : swiglu_bwd_packed_kernel<false>;
+    const int units = static_cast<int>(cols / 16), rpb = kRowsPerBlock * units <= kUnitsPerBlock ? kRowsPerBlock : kUnitsPerBlock / units;
+    const int64_t blocks = (rows + rpb - 1) / rpb;
+    kernel<<<static_cast<unsigned>(blocks < (1 << 30) ? blocks : (1 << 30)), 256, row_grad_out ? sizeof(float) * rpb * units : 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const int8_t*>(gate_q), gate_scales, static_cast<const int8_t*>(up_q), up_scales, static_cast<const __nv_bfloat16*>(d_hidden),
         static_cast<__nv_bfloat16*>(d_gate), static_cast<__nv_bfloat16*>(d_up), static_cast<__nv_bfloat16*>(hidden), row_scale, row_grad_out,
-        num_rows, rows, static_cast<int>(cols), static_cast<int>((cols + kBlock - 1) / kBlock), has_limit, limit);
+        num_rows, rows, static_cast<int>(cols), static_cast<int>((cols + kBlock - 1) / kBlock), rpb, limit);
     MOKB_CUDA(cudaGetLastError());
     note_launch();
     return MOKB_OK;

@@ -259,7 +259,7 @@ def swiglu_bwd_packed_op(
     num_rows: torch.Tensor | None = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """The backward pass of hidden = silu(gate) * up from packed gate and up: d_gate, d_up, hidden (bf16) and per row
-    sum(d_hidden * hidden) / row_scale (0 where row_scale is not positive; without row_scale, the sum)."""
+    sum(d_hidden * hidden) / row_scale (0 where row_scale is not positive; without row_scale, the sum). At most 131072 columns."""
     shape = _check_packed("gate_q", gate_q, gate_scales)
     if _check_packed("up_q", up_q, up_scales, gate_q.device) != shape:
         raise ValueError("gate and up must have the same shape")

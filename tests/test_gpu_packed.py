@@ -110,6 +110,30 @@ def test_swiglu_backward(size, limit):
         assert ((got[3].double() - want[3]).abs() <= (c + 128) * P.U32 * total + lost.sum(1) * (1 + inv)).all()
 
 
+@pytest.mark.parametrize("size", [(5, 131072), (11, 16400), (3, 32784), (2049, 16), (257, 4080)], ids=lambda s: "x".join(map(str, s)))
+def test_swiglu_backward_wide_and_narrow_rows(size):
+    """Rows wider than a block's shared memory holds eight of, and units that straddle 128 values; each row's results are the row's alone."""
+    from mok import ops
+    n, c = size
+    gen = torch.Generator(device="cuda").manual_seed(n * c)
+    gate, up, dh = (torch.randn(n, c, generator=gen, device="cuda").bfloat16() for _ in range(3))
+    gp, upk = ops.pack_rows(gate), ops.pack_rows(up)
+    w = torch.rand(n, generator=gen, device="cuda") + 0.5
+    got = ops.swiglu_bwd_packed(*gp, *upk, dh, None, w)
+    g, u, d = P.pack(gate)[2].double(), P.pack(up)[2].double(), dh.double()
+    want = P.swiglu_bwd(g, u, d, None, w)
+    sig = torch.sigmoid(g)
+    terms = ((sig + (g * sig).abs() * (1 + sig)) * u.abs() * d.abs(), want[1].abs(), want[2].abs())       # as in test_swiglu_backward
+    for a, b, e in zip(got[:3], want[:3], terms):
+        assert ((a.double() - b).abs() <= 128 * P.U32 * e + P.U16 * (b.abs() + 128 * P.U32 * e)).all()
+    total = (dh.double() * want[2]).abs().sum(1) / w.double()
+    assert ((got[3].double() - want[3]).abs() <= (c + 128) * P.U32 * total).all()
+    for row in (0, n // 2, n - 1):
+        one = [t[row:row + 1].contiguous() for t in (*gp, *upk, dh)]
+        alone = ops.swiglu_bwd_packed(*one, None, w[row:row + 1].contiguous())
+        assert all(torch.equal(a[0], b[row]) for a, b in zip(alone, got))
+
+
 def test_gradient_against_differences():
     from mok import ops
     gen = torch.Generator(device="cuda").manual_seed(2)

@@ -141,6 +141,7 @@ def test_the_library_checks_sizes_and_addresses():
     refused(lib.mokb_unpack_rows(a, a, a, None, -1, 128, None), b"multiple of 16")
     refused(lib.mokb_swiglu_bwd_packed(a, a, a, a, a, a, a, None, None, None, None, 4, 128, 0, 0.0, None), b"null")
     refused(lib.mokb_swiglu_bwd_packed(a, a, a, a, a, a, a, ctypes.c_void_p(4112), None, None, None, 4, 128, 0, 0.0, None), b"aligned")
+    refused(lib.mokb_swiglu_bwd_packed(a, a, a, a, a, a, a, a, None, None, None, 4, 131088, 0, 0.0, None), b"131072")
     assert lib.mokb_pack_rows(None, None, None, None, 0, 128, None) == 0
     b = _C.BwdArgs()
     refused(lib.mokb_dispatch_mlp_swiglu_combine_bwd_bf16_packed(ctypes.byref(b), None, None), b"null packed context")
