@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         for (int i = 0; i < PER; ++i) {
             const int e = expert_of<VEC>(i, lane);
             float order = v[i];
-            if (SIGMOID && p.bias && order > -INFINITY && e < p.E) order = sigmoid(order) + __ldg(p.bias + e);
+            if (SIGMOID && p.bias && order > -INFINITY && e < p.E) order = clean(sigmoid(order) + __ldg(p.bias + e));      // (a NaN's key could be none)
             key[i] = e >= p.E ? 0u : (order_key(order) & ~kIndex) | (kIndex - static_cast<uint32_t>(e));
         }
         int mine;                            // lane k: the k-th pick
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
                     uint32_t exact = 0u;
                     if (e < p.E) {
                         const double l = load_clean<BF16>(p, row, e);
-                        exact = l == -INFINITY ? kClosedKey : order_key(static_cast<float>(1.0 / (1.0 + exp(-l)) + static_cast<double>(p.bias[e])));
+                        exact = l == -INFINITY ? kClosedKey : order_key(clean(static_cast<float>(1.0 / (1.0 + exp(-l)) + static_cast<double>(p.bias[e]))));
                     }
 #pragma unroll
                     for (int j = 0; j < PER; ++j)

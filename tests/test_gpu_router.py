@@ -272,3 +272,20 @@ def test_a_row_whose_order_needs_64_bits():
     close = 1.0 + torch.randint(0, 16, (300, E), generator=gen, device="cuda").float() * 2.0 ** -23
     check_forward(F.MoKRouterConfig(topk=K), close)
     check_forward(F.MoKRouterConfig(topk=K), -close)
+
+
+def test_a_bias_that_is_no_number_comes_last():
+    """E = topk takes every expert, whatever the bias holds; picks stay different experts of the row."""
+    from mok import functional as F
+    for E, K in ((8, 8), (40, 32), (64, 6), (200, 5)):
+        logits = logits_of(30, E, torch.float32, seed=E)
+        bias = torch.zeros(E, device="cuda")
+        bias[0], bias[3], bias[5] = math.nan, -math.inf, math.inf
+        r = F.route(F.MoKRouterConfig(topk=K, score="sigmoid"), logits, bias, balance=True)
+        order = torch.sigmoid(logits.double()).add(bias.double())
+        order[:, 0] = -math.inf
+        want = torch.sort(order, dim=1, descending=True, stable=True).indices[:, :K]
+        assert torch.equal(r.top_experts, want)
+        s = torch.sigmoid(logits.double()).gather(1, want)
+        assert ((r.router_weights.double() - s / s.sum(1, keepdim=True)).abs() <= (K + 64) * U).all()
+        assert int(r.tokens_per_expert.sum()) == 30 * K
