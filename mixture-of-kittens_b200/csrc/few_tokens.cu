@@ -581,7 +581,8 @@ __global__ void __launch_bounds__(kThreads, 1) few_product_kernel(const __grid_c
             // the tile's other part), and then its sums never leave tensor memory.
             const int c_lo = g.k0 == 0 && g.k1 == g.ks ? cta : st.owner(g.first), c_hi = c_lo == cta && g.k1 == g.ks ? cta : st.owner(g.first + g.ks - 1);
             int32_t* const ticket = p.w.counters + (DOWN ? p.sms : 0) + c_lo;
-            if (!mbar_wait(tfull_bar(buf), (local >> 1) & 1u, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT)) break;
+            // (a wait that ran out has set the status word, so what follows is void, but the barriers below need all eight warps)
+            mbar_wait(tfull_bar(buf), (local >> 1) & 1u, abort_flag, p.status, MOKB_ST_PIPELINE_TIMEOUT);
             tc_fence_after();
             const uint32_t t0 = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + buf * 2 * acc_cols, t1 = t0 + acc_cols;
             bool mine_in_tmem = true;
