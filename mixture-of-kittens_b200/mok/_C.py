@@ -587,6 +587,11 @@ def route_bwd(logits, top_experts, d_router_weights, d_score_sums, sigmoid, reno
     return d_logits
 
 
+def _f32(limit):
+    """A limit as a number that fits 32 bits: beyond their range it limits nothing."""
+    return 0.0 if limit is None else float(limit) if limit < 3.4e38 else float("inf")
+
+
 def few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w_shared_down, w_routed_gate, w_routed_up,
                    w_routed_down, scales, first_expert, swiglu_limit):
     """`scales`: None, or the packed scales of the three routed weights (MXFP8).  The work area is a tensor of this call:
@@ -599,7 +604,7 @@ def few_tokens_fwd(x, top_experts, router_weights, w_shared_gate, w_shared_up, w
     gs, us, ds = (scales[0].data_ptr(), scales[1].data_ptr(), scales[2].data_ptr()) if mx else (0, 0, 0)
     y = torch.empty_like(x)
     work = torch.empty(lib.mokb_few_tokens_workspace_bytes(T, H, I, K, mx), dtype=torch.uint8, device=x.device)
-    args = _pack_few(T, H, I, E, K, first_expert, mx, swiglu_limit is not None, swiglu_limit or 0.0, x.data_ptr(), top_experts.data_ptr(),
+    args = _pack_few(T, H, I, E, K, first_expert, mx, swiglu_limit is not None, _f32(swiglu_limit), x.data_ptr(), top_experts.data_ptr(),
                      router_weights.data_ptr(), sg, su, sd, w_routed_gate.data_ptr(), w_routed_up.data_ptr(), w_routed_down.data_ptr(),
                      gs, us, ds, y.data_ptr(), work.data_ptr(), status_tensor(x.device).data_ptr())
     _ck(_few_tokens_fwd_packed(args, _stream()))

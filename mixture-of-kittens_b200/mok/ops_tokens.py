@@ -2,8 +2,6 @@
 kept in 8 bits between the forward and the backward pass.  The reference has none of them (its layer starts from given routes,
 takes 512 tokens or more and saves bf16 or MXFP8); the manner is that of its other operators: arguments are checked before any
 device work (ValueError / TypeError), outputs are allocated, nothing synchronises the host.  `mok.ops` re-exports them."""
-import math
-
 import torch
 
 from . import _C
@@ -17,6 +15,7 @@ MAX_ROUTE_TOPK = 32
 PACK_BLOCK = _C.PACK_BLOCK
 
 BF16, F32, I64 = torch.bfloat16, torch.float32, torch.int64
+FLT_MAX = torch.finfo(torch.float32).max
 
 
 def _check_cuda(name: str, t: torch.Tensor, dtype, shape=None, device=None, contiguous=True) -> None:
@@ -60,8 +59,8 @@ def check_route_knobs(topk, score, renormalize, scale) -> None:
         raise ValueError("score must be 'softmax' or 'sigmoid'")
     if type(renormalize) is not bool:
         raise TypeError("renormalize must be a boolean")
-    if type(scale) not in (int, float) or not math.isfinite(scale):
-        raise ValueError("scale must be a finite number")
+    if type(scale) not in (int, float) or not abs(scale) <= FLT_MAX:
+        raise ValueError("scale must be a finite number of fp32's range")
 
 
 def _check_logits(logits, topk, score, renormalize, scale) -> tuple[int, int]:
@@ -87,7 +86,7 @@ def route(logits, bias, topk, score, renormalize, scale, balance):
     fp32 and, with `balance`, tokens_per_expert [E] int32 and score_sums [E] fp32 (else None, None).
 
     score "softmax": the largest logits are picked; "sigmoid": the largest 1 / (1 + exp(-logit)) + bias (`bias` [E] fp32, finite,
-    only picks, has no gradient).  Weights are the scores of the picks times `scale`, with `renormalize` divided by their sum.
+    only picks, has no gradient; where the sum is NaN or -inf the expert comes last).  Weights are the scores of the picks times `scale`, with `renormalize` divided by their sum.
     Ties go to the lowest index.  Logits that are -inf or NaN close an expert for the token: picked only when nothing else is left,
     with weight 0; not counted in the load figures."""
     T, E = _check_logits(logits, topk, score, renormalize, scale)

@@ -1,4 +1,6 @@
 """The layer for a few tokens against a plain implementation in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -216,3 +218,11 @@ def test_router_feeds_both_forms_of_the_layer():
     # the other form also rounds gate, up and every expert's result to bf16, and both round hidden and y: at most eight roundings of a
     # factor of y, of random sign; four worst cases cover their sum
     assert (whole.double() - torch.cat(pieces).double()).norm() <= 4 * P.U16 * ref.norm()
+
+
+def test_a_limit_beyond_fp32_limits_nothing():
+    from mok import functional as F
+    x, e, w, shared, routed = make(5, 256, 128, 4, 2, seed=12)
+    want = F.forward_few_tokens(x, e, w, *shared, *routed)
+    for limit in (1e300, math.inf, 10 ** 40):
+        assert torch.equal(F.forward_few_tokens(x, e, w, *shared, *routed, limit), want)

@@ -19,7 +19,8 @@ def test_router_arguments():
         call()
     for kw, error, why in (
             (dict(topk=0), ValueError, "topk"), (dict(topk=33), ValueError, "topk"), (dict(topk=17), ValueError, "num_experts"),
-            (dict(score="relu"), ValueError, "score"), (dict(scale=float("nan")), ValueError, "scale"),
+            (dict(score="relu"), ValueError, "score"), (dict(scale=float("nan")), ValueError, "scale"), (dict(scale=-float("inf")), ValueError, "scale"),
+            (dict(scale=1e39), ValueError, "scale"),
             (dict(logits=torch.zeros(4, 1025)), ValueError, "num_experts"), (dict(logits=torch.zeros(16)), ValueError, "shape"),
             (dict(logits=torch.zeros(4, 16, dtype=torch.float16)), TypeError, "dtype"), (dict(logits=l.double()), TypeError, "dtype")):
         with pytest.raises(error, match=why):
