@@ -127,7 +127,7 @@ __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.N
 // to a block: 509, sixteen: 450); one launch at 25088 x 1408 with a limit: 68 us (73, 77, 94, 70).  Held to 48 registers, a few of which
 // spill: with 64, 75 and 480 to 500 us, with 40, 80 and 482.
 // Back to back it is the board's power that bounds it (1 kW, 1.6 of 1.97 GHz), so instructions count: the sigmoid's quotient is the
-// approximate one, 2 steps of fp32 off where bf16 keeps 2^15 of them (IEEE: 500).
+// approximate one, off by 2 steps of fp32, of which a step of bf16 is 65536 (IEEE: 500 us).
 constexpr int kRowsPerBlock = 8, kUnitsPerBlock = 8192;
 template <bool LIMIT>
 __global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
