@@ -14,13 +14,15 @@
 // has given both looks for its next two.  For bf16 logits nothing is lost by that.  For fp32 ones the order of two that agree in all other
 // bits is open: where that happens between neighbours in the order of the picks (the first that is left out among them), the row is done
 // again by key and index.  With a bias the keys are s + bias, and two of them a rounding apart must not change places with how exp is
-// evaluated: the order is that of the sums worked out in 64 bits and rounded to 32.  They too are first picked in 32 bits, and the row is
-// done again in 64 where neighbours are nearer than the error of that.
+// evaluated: the order is that of the sums worked out in 64 bits and rounded to 32.  They too are first picked by such keys; then the picks'
+// own sums in 32 bits, and the most that the next key can stand for, say whether that was the order, and the row is done again in 64 where
+// neighbours are nearer than the error of that.  (Asking the keys themselves, short of seven bits and more, sends 6 % of the rows there at
+// 128 experts: 28 us instead of 26; at 512 experts 57 instead of 39.)
 // (16384 x 256, 8 picks: 28 us looking through all keys for every pick, 19 with keys and indices apart.)
 //
-// Bound by instruction issue at long micro-batches (60 to 77 % of the cycles issue, memory at a tenth of its rate).  16384 x 256 in fp32, 8 picks with
-// load figures: 17.5 us forward, 7 for the sum of the figures (begun in the forward's end), 11.6 backward; 32768 x 128 with a bias: 27, 8 and 13.
-// The logits alone take 2.6 us.
+// Bound by instruction issue at long micro-batches (60 to 77 % of the cycles issue, memory at a tenth of its rate).  Graph replays back to back:
+// 16384 x 256 in fp32, 8 picks: 11.8 us forward, 17.2 with the load figures, 8.7 backward; 32768 x 128 with a bias: 21.6, 26 and 10.3; 16384 x 512
+// with a bias: 34, 39 and 10.4.  The logits alone take 2.6 to 5.1 us.
 #include <float.h>
 
 #include "common.cuh"
@@ -127,50 +129,36 @@ __device__ __forceinline__ float score_of(float l, float top, float inv_total) {
 
 constexpr int index_bits(int per) { return per == 4 ? 7 : per == 8 ? 8 : per == 16 ? 9 : 10; }
 
-// The topk largest keys, indices in their low bits, in falling order: lane k returns the k-th one's expert.  CHECK: one more is looked for,
-// and *open says whether the order of two neighbours is not settled (closed experts always are): keys that differ only in the index, or
-// (BIASED) sums that are nearer than their errors.
-template <int PER, bool CHECK, bool BIASED>
-__device__ __forceinline__ int pick(const uint32_t (&key)[PER], int K, int lane, bool* open) {
-    constexpr int B = index_bits(PER);
-    uint32_t b1, b2, mine = 0u, last = 0u;        // b1, b2: this lane's two largest that are not taken
+// The topk largest keys, indices in their low bits, in falling order: lane k has the k-th one in *mine.  NEXT: *next is the one that follows.
+template <int PER, bool NEXT>
+__device__ __forceinline__ void pick(const uint32_t (&key)[PER], int K, int lane, uint32_t* mine, uint32_t* next) {
+    uint32_t b1 = 0u, b2 = 0u, last = 0u;         // b1, b2: this lane's two largest that are not taken
     int cached = 2;
-    auto look = [&](uint32_t below) {
-        b1 = b2 = 0u;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint32_t k = key[i] < below ? key[i] : 0u;
-            b2 = max(b2, min(b1, k));
-            b1 = max(b1, k);
-        }
-    };
-    look(0xffffffffu);
-    const int rounds = CHECK ? K + 1 : K;
+    for (int i = 0; i < PER; ++i) {
+        b2 = max(b2, min(b1, key[i]));
+        b1 = max(b1, key[i]);
+    }
+    *mine = 0u;
+    const int rounds = NEXT ? K + 1 : K;
     for (int k = 0; k < rounds; ++k) {
         last = __reduce_max_sync(0xffffffffu, b1);
-        if (lane == k) mine = last;
+        if (lane == k) *mine = last;
         if (b1 == last) {
             b1 = b2;
             if (--cached == 0) {
-                look(last);
+                b1 = b2 = 0u;
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const uint32_t below = key[i] < last ? key[i] : 0u;
+                    b2 = max(b2, min(b1, below));
+                    b1 = max(b1, below);
+                }
                 cached = 2;
             }
         }
     }
-    if (CHECK) {
-        uint32_t below = __shfl_down_sync(0xffffffffu, mine, 1);
-        if (lane == K - 1) below = last;
-        bool unsettled;
-        if (BIASED) {
-            // both keys lost up to 2^(B - 23) of their size to the index
-            const float hi = key_value(mine), lo = key_value(below);
-            unsettled = hi - lo <= 1e-6f + (1e-6f + 2.0f / (1 << (22 - B))) * fmaxf(fabsf(hi), fabsf(lo));
-        } else {
-            unsettled = ((mine ^ below) >> B) == 0u;
-        }
-        *open = __any_sync(0xffffffffu, lane < K && (below >> B) > (kClosedKey >> B) && unsettled);
-    }
-    return ((1 << B) - 1) - static_cast<int>(mine & ((1u << B) - 1u));
+    *next = last;
 }
 // The same by key and index, for rows whose order that leaves open.
 template <int PER, bool VEC>
@@ -225,47 +213,56 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         for (int i = 0; i < PER; ++i) {
             const int e = expert_of<VEC>(i, lane);
             float order = v[i];
-            if (SIGMOID && p.bias && order > -INFINITY && e < p.E) order = clean(sigmoid(order) + __ldg(p.bias + e));      // (a NaN's key could be none)
+            if (SIGMOID && p.bias) {
+                v[i] = sigmoid(order);       // (0 where closed)
+                if (order > -INFINITY && e < p.E) order = clean(v[i] + __ldg(p.bias + e));      // (a NaN's key could be none)
+            }
             key[i] = e >= p.E ? 0u : (order_key(order) & ~kIndex) | (kIndex - static_cast<uint32_t>(e));
         }
-        int mine;                            // lane k: the k-th pick
+        constexpr bool kExact = BF16 && !SIGMOID;      // (a bf16 logit's key loses nothing to the index)
+        uint32_t mine_key, next_key;
+        pick<PER, !kExact>(key, p.K, lane, &mine_key, &next_key);
+        int mine = static_cast<int>(kIndex - (mine_key & kIndex));      // lane k: the k-th pick
+        float l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
         if (SIGMOID && p.bias) {
-            // s in 32 bits: an exp (off by some 2 + 1.2 |l| units in the last place; s (1 - s) <= 1/4 and |l| s (1 - s) < 0.23 of that), a sum
-            // and a quotient: below 3e-7.  s + bias and the 32-bit form of the exact sum are rounded once each.  Two neighbours that are
-            // more than 1e-6 (1 + |s + bias|) apart are in order.
-            bool open;
-            mine = pick<PER, true, true>(key, p.K, lane, &open);
-            if (open) {
+            // The picks' sums as they are, and the largest that one which is left out can be.  s in 32 bits: an exp (off by some 2 + 1.2 |l|
+            // units in the last place; s (1 - s) <= 1/4 and |l| s (1 - s) < 0.23 of that), a sum and a quotient: below 3e-7.  s + bias and the
+            // 32-bit form of the exact sum are rounded once each.  Neighbours that are more than 1e-6 (1 + |s + bias|) apart are in order.
+            const float hi = l > -INFINITY ? clean(sigmoid(l) + __ldg(p.bias + mine)) : -INFINITY;
+            float lo = __shfl_down_sync(0xffffffffu, hi, 1);
+            if (lane == p.K - 1) lo = (next_key | kIndex) > kClosedKey ? key_value(next_key | kIndex) : -INFINITY;
+            const bool unsettled = lane < p.K && lo > -INFINITY && !(hi - lo > 1e-6f + 1e-6f * fmaxf(fabsf(hi), fabsf(lo)));
+            if (__any_sync(0xffffffffu, unsettled)) {
 #pragma unroll 1
                 for (int i = 0; i < PER; ++i) {
                     const int e = expert_of<VEC>(i, lane);
                     uint32_t exact = 0u;
                     if (e < p.E) {
-                        const double l = load_clean<BF16>(p, row, e);
-                        exact = l == -INFINITY ? kClosedKey : order_key(clean(static_cast<float>(1.0 / (1.0 + exp(-l)) + static_cast<double>(p.bias[e]))));
+                        const double x = load_clean<BF16>(p, row, e);
+                        exact = x == -INFINITY ? kClosedKey : order_key(clean(static_cast<float>(1.0 / (1.0 + exp(-x)) + static_cast<double>(p.bias[e]))));
                     }
 #pragma unroll
                     for (int j = 0; j < PER; ++j)
                         if (j == i) key[j] = exact;
                 }
                 mine = pick_by_key_and_index<PER, VEC>(key, p.K, lane);
+                l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
             }
-        } else if (BF16) {
-            mine = pick<PER, false, false>(key, p.K, lane, nullptr);
-        } else {
-            bool open;
-            mine = pick<PER, true, false>(key, p.K, lane, &open);
-            if (open) {
+        } else if (!BF16) {
+            uint32_t below = __shfl_down_sync(0xffffffffu, mine_key, 1);
+            if (lane == p.K - 1) below = next_key;
+            // keys that differ only in the index (closed experts are in order by that)
+            if (__any_sync(0xffffffffu, lane < p.K && (below | kIndex) > kClosedKey && (mine_key | kIndex) == (below | kIndex))) {
 #pragma unroll
                 for (int i = 0; i < PER; ++i) key[i] = expert_of<VEC>(i, lane) < p.E ? order_key(v[i]) : 0u;
                 mine = pick_by_key_and_index<PER, VEC>(key, p.K, lane);
+                l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
             }
         }
-        const float l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
         float inv_total = 1.0f, top = 0.0f;
         if (!SIGMOID) top = __shfl_sync(0xffffffffu, l, 0);          // the first pick has the largest logit
         if (balance || (!SIGMOID && !p.renormalize)) {
-            const float total = exponentials<PER, SIGMOID>(v, top);
+            const float total = SIGMOID && p.bias ? 1.0f : exponentials<PER, SIGMOID>(v, top);
             if (!SIGMOID) inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
             if (balance) {
 #pragma unroll
