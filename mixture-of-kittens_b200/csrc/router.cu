@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         const int e = expert_of<VEC>(i, lane);
         ds_sm[e] = p.d_score_sums && e < p.E ? __ldg(p.d_score_sums + e) : 0.0f;
     }
+    __syncwarp();          // (a pick's number is read by the lane of the pick, not by the one that has filled it in)
     const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
     int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp;
     float next[PER];
