@@ -85,8 +85,8 @@ struct Work {
 };
 
 inline size_t align256(size_t x) { return (x + 255) / 256 * 256; }
-inline int column_cap(int T, bool mx) {
-    const int n = (T + 15) / 16 * 16;
+inline int column_cap(int T, bool mx) {      // (16 for an empty step too, whose work area is asked for like any other's)
+    const int n = T > 0 ? (T + 15) / 16 * 16 : 16;
     return n < unit_columns(mx) ? n : unit_columns(mx);
 }
 inline int max_units(int T, int K, bool mx) { return T * K + T / column_cap(T, mx) + 2; }      // a routed unit has a route; shared ones
