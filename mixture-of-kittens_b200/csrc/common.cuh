@@ -274,6 +274,14 @@ __device__ __forceinline__ bool index_ok(const IndexGuard& g, int idx, int kind,
     return false;
 }
 
+// ---- a row's router-weight gradient, sum(d_hidden * hidden) / w: 1 / w goes into every term (d_hidden holds w, so that d_hidden * hidden alone
+// can be below fp32's range), and is past that range for a weight of 2^-128 or less, where it would make NaN of every zero.  So such
+// weights are taken times 2^64 (row_inverse) and the sum is multiplied by that (row_rest); for all others row_rest is 1.  No weight, or
+// one that is not positive: 0.
+__device__ __forceinline__ bool tiny_weight(float w) { return w > 0.0f && w <= 0x1p-128f; }
+__device__ __forceinline__ float row_inverse(float w) { return w > 0.0f ? 1.0f / (tiny_weight(w) ? w * 0x1p64f : w) : 0.0f; }
+__device__ __forceinline__ float row_rest(float w) { return tiny_weight(w) ? 0x1p64f : 1.0f; }
+
 // ---- programmatic dependent launch: a kernel launched with launch_after() (below) may start once every block of the kernel before it has
 // called grid_dep_launch() or ended; what it needs of that kernel's results it reads after grid_dep_wait(), which returns when that kernel
 // is complete.  (Both do nothing in a kernel that is launched otherwise.)

@@ -72,11 +72,8 @@ __global__ void swiglu_bwd_kernel(const uint4* __restrict__ gate, const uint4* _
     const int wpb = blockDim.x >> 5;
     const int64_t nwarps = static_cast<int64_t>(gridDim.x) * wpb;
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * wpb + (threadIdx.x >> 5); row < rows; row += nwarps) {
-        float inv_w = 1.0f;
-        if (row_grad_out) {
-            const float w = row_scale ? row_scale[row] : 1.0f;
-            inv_w = w > 0.0f ? 1.0f / w : 0.0f;
-        }
+        const float w = row_grad_out && row_scale ? row_scale[row] : 1.0f;
+        const float inv_w = row_inverse(w);
         float partial = 0.0f;
         const int64_t base = row * vec_per_row;
         for (int v = lane; v < vec_per_row; v += 32) {
@@ -103,7 +100,7 @@ __global__ void swiglu_bwd_kernel(const uint4* __restrict__ gate, const uint4* _
         if (row_grad_out) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) partial += __shfl_xor_sync(0xffffffffu, partial, o);
-            if (lane == 0) row_grad_out[row] = partial;
+            if (lane == 0) row_grad_out[row] = partial * row_rest(w);
         }
     }
 }

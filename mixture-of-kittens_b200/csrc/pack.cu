@@ -150,11 +150,7 @@ __global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
             const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
             uint32_t og[8], ou[8], oh[8];
             float sum = 0.0f;
-            float inv_w = 1.0f;
-            if (row_grad && row_scale) {
-                const float w = __ldg(row_scale + row0 + r);
-                inv_w = w > 0.0f ? 1.0f / w : 0.0f;
-            }
+            const float inv_w = row_grad && row_scale ? row_inverse(__ldg(row_scale + row0 + r)) : 1.0f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float g4[4], u4[4], dg[4], du[4], h[4];
@@ -193,7 +189,7 @@ __global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
                 for (int u = threadIdx.x & 31; u < units; u += 32) sum += unit_sum[r * units + u];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if ((threadIdx.x & 31) == 0) row_grad[row0 + r] = sum;
+                if ((threadIdx.x & 31) == 0) row_grad[row0 + r] = row_scale ? sum * row_rest(__ldg(row_scale + row0 + r)) : sum;
             }
             __syncthreads();
         }

@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(256, 2) swiglu_bwd_quant_kernel(
         if (k < 3) next = fetch(k + 1);
         const int64_t row = r0 + rr + 32 * k;
         const float gs = __uint_as_float(o.gs << 23), us = __uint_as_float(o.us << 23);
-        const float inv_w = o.w > 0.0f ? 1.0f / o.w : 0.0f;
+        const float inv_w = row_inverse(o.w);
         const uint32_t gv[4] = {o.g.x, o.g.y, o.g.z, o.g.w}, uv[4] = {o.u.x, o.u.y, o.u.z, o.u.w};
         uint32_t wg[8], wu[8];
         float rg_a[16], rg_b[16];          // factors of the row gradient's terms
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256, 2) swiglu_bwd_quant_kernel(
                 for (int i = 0; i < 16; ++i) run = fmaf(rg_a[i], rg_b[i], run);
             }
             const float upper = __shfl_down_sync(0xffffffffu, run, 4);
-            if (seg == 3) partials[row * (I >> 7) + blockIdx.x] = run + upper;
+            if (seg == 3) partials[row * (I >> 7) + blockIdx.x] = (run + upper) * row_rest(o.w);
         }
     }
     __syncthreads();

@@ -1,0 +1,90 @@
+"""The backward pass of SwiGLU (whole, packed and quantising) at weights where 1 / w leaves fp32's range."""
+import pytest
+import torch
+
+from tests import plain_forms as P
+
+pytestmark = pytest.mark.gpu
+
+
+TINY = [1e-45, 1e-42, 1e-39, 2.0 ** -128, 2.0 ** -127, 2.0 ** -126, 1e-30, 0.5]
+
+
+def rows_with_zeros(n, c, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    gate, up, dh = (torch.randn(n, c, generator=gen, device="cuda").bfloat16() for _ in range(3))
+    gate[:, 1::5] = 0.0
+    dh[:, 2::7] = 0.0
+    return gate, up, dh
+
+
+def check_row_gradient(got, gate, up, dh, w):
+    """sum(d_hidden * hidden) / w of d_hidden that is as small as w: c products and a sum in fp32 of terms that the rows' weights bring
+    back to ordinary size, a quotient, and silu's own roundings (as test_gpu_packed.py counts them)."""
+    c = gate.shape[1]
+    terms = dh.double() * (gate * torch.sigmoid(gate) * up)
+    want = torch.where(w > 0, terms.sum(1) / torch.where(w > 0, w, 1.0).double(), 0.0)
+    room = torch.where(w > 0, terms.abs().sum(1) / torch.where(w > 0, w, 1.0).double(), 0.0)
+    assert torch.isfinite(got).all(), got
+    assert ((got.double() - want).abs() <= (c + 128) * P.U32 * room).all(), (got, want)
+
+
+def scaled(dh, w):
+    """d_hidden of rows scaled by their weights: bf16, exact where the product is a normal number."""
+    return (dh.double() * w.double()[:, None]).bfloat16()
+
+
+def test_row_gradient_of_tiny_weights_packed():
+    from mok import ops
+    w = torch.tensor(TINY, device="cuda")
+    gate, up, dh = rows_with_zeros(len(TINY), 512)
+    dh = scaled(dh, w)
+    gp, upk = ops.pack_rows(gate), ops.pack_rows(up)
+    got = ops.swiglu_bwd_packed(*gp, *upk, dh, None, w)[3]
+    check_row_gradient(got, P.pack(gate)[2], P.pack(up)[2], dh, w)
+
+
+def test_row_gradient_of_tiny_weights_whole():
+    from mok import _C
+    w = torch.tensor(TINY, device="cuda")
+    gate, up, dh = rows_with_zeros(len(TINY), 512)
+    dh = scaled(dh, w)
+    got = _C.swiglu_bwd(gate, up, dh, None, w, True)[2]
+    check_row_gradient(got, gate.double(), up.double(), dh, w)
+
+
+@pytest.mark.parametrize("precision", ["bf16", "packed", "mxfp8"])
+def test_router_gradients_of_the_layer_at_tiny_weights(precision):
+    """Routes whose weight is positive but below 2^-128 (a softmax that is not renormalised has such): their scaled rows underflow, and
+    the router's gradient stays a number.  Every other route's gradients are as in a run without them."""
+    from mok import _C, functional as F, ops
+    from oracle import mok_oracle as O
+    from tests.gpu_common import init_single_rank_group, to_dev
+    T, H, I, E, K = 512, 512, 256, 8, 2
+    inp = to_dev(O.make_inputs(R=1, T=T, H=H, I=I, E=E, K=K, seed=33, routing="router")[0])
+    cfg = F.MoKConfig(minibatch_size=256, macrobatch_size=(T * K + E * 256 + 255) // 256 * 256, schedule_capacity_multiplier=4.0)
+    ws = F.create_workspace(cfg, init_single_rank_group(), device=torch.device("cuda", 0), num_local_tokens=T, hidden_size=H, topk=K)
+    sched = F.build_schedule(ws, cfg, inp.top_experts, num_local_experts=E)
+    shared = (inp.w_shared_gate, inp.w_shared_up, inp.w_shared_down)
+    routed = bwd = (inp.w_routed_gate, inp.w_routed_up, inp.w_routed_down)
+    if precision == "mxfp8":
+        q = [ops.mxfp8_quantize(t, True, True) for t in routed]
+        routed = tuple(t[:2] for t in q)
+        bwd = (q[0], q[1], q[2][2:])
+
+    def gradients(weights):
+        _, ctx = F.forward(cfg, ws, sched, inp.x, weights, *shared, *routed)
+        if precision == "packed":
+            ctx = F.pack_context(sched, ctx)
+        grads = F.backward(cfg, ws, sched, ctx, inp.grad_output, inp.x, weights, *shared, *bwd)
+        torch.cuda.synchronize()
+        assert _C.check_status() == 0
+        return grads
+    plain = gradients(inp.router_weights)
+    weights = inp.router_weights.clone()
+    weights[::3, 1] = 1e-42
+    weights[1::3, 0] = 1e-39
+    d_x, d_w = gradients(weights)[:2]
+    assert torch.isfinite(d_w).all() and torch.isfinite(d_x).all()
+    same = weights == inp.router_weights
+    assert torch.equal(d_w[same], plain[1][same])
