@@ -561,7 +561,8 @@ int mokb_route_bwd(const void* logits, int bf16, int64_t row_stride, int64_t num
  * with an infinity or NaN come back as NaN.  With num_rows (device, optional) only rows [0, min(*num_rows, rows)) are read and
  * written, in all three.  Alignment: bf16 tensors 32 bytes, q 16.
  * mokb_swiglu_bwd_packed: mokb_swiglu_bwd from packed gate and up, not rounded to bf16 in between; it also writes hidden
- * [rows, cols]; cols at most 131072.  Outputs must not overlap inputs. */
+ * [rows, cols]; cols at most 131072.  row_grad_out is 0 for rows whose row_scale is not positive, whatever they hold.  Outputs must
+ * not overlap inputs. */
 int mokb_pack_rows(const void* x, void* q, float* scales, const int32_t* num_rows, int64_t rows, int64_t cols, void* stream);
 int mokb_unpack_rows(const void* q, const float* scales, void* x, const int32_t* num_rows, int64_t rows, int64_t cols, void* stream);
 int mokb_swiglu_bwd_packed(const void* gate_q, const float* gate_scales, const void* up_q, const float* up_scales,

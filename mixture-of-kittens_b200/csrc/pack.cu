@@ -189,7 +189,10 @@ __global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
                 for (int u = threadIdx.x & 31; u < units; u += 32) sum += unit_sum[r * units + u];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if ((threadIdx.x & 31) == 0) row_grad[row0 + r] = row_scale ? sum * row_rest(__ldg(row_scale + row0 + r)) : sum;
+                if ((threadIdx.x & 31) == 0) {
+                    const float w = row_scale ? __ldg(row_scale + row0 + r) : 1.0f;
+                    row_grad[row0 + r] = w > 0.0f ? sum * row_rest(w) : 0.0f;      // (0 times a fault in the row would be NaN)
+                }
             }
             __syncthreads();
         }

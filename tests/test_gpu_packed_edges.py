@@ -1,4 +1,6 @@
-"""The backward pass of SwiGLU (whole, packed and quantising) at weights where 1 / w leaves fp32's range."""
+"""The backward pass of SwiGLU (whole, packed and quantising) at weights where 1 / w leaves fp32's range, and at rows without a weight."""
+import math
+
 import pytest
 import torch
 
@@ -88,3 +90,21 @@ def test_router_gradients_of_the_layer_at_tiny_weights(precision):
     assert torch.isfinite(d_w).all() and torch.isfinite(d_x).all()
     same = weights == inp.router_weights
     assert torch.equal(d_w[same], plain[1][same])
+
+
+def test_a_row_without_a_weight_has_no_row_gradient():
+    """0 where row_scale is not positive (or not a number), whatever the row holds: a block that came back as NaN, a product past
+    fp32's range, an infinite d_hidden."""
+    from mok import ops
+    c = 256
+    gate, up, dh = (torch.ones(8, c, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    gate[0, 3] = math.nan
+    up[1, 200] = -math.inf
+    gate[2], up[2] = 3e38, 3e38
+    dh[3, 5] = math.inf
+    dh[4, 6] = math.nan
+    w = torch.tensor([0.0, -0.0, 0.0, -1.0, 0.0, math.nan, -math.inf, 1.0], device="cuda")
+    for limit in (None, 7.0):
+        got = ops.swiglu_bwd_packed(*ops.pack_rows(gate), *ops.pack_rows(up), dh, limit, w)[3]
+        assert (got[:7] == 0).all(), got
+        assert torch.isfinite(got[7]) and got[7] > 0
