@@ -123,11 +123,11 @@ __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.N
 
 // A block takes up to eight consecutive rows, its threads their units in order, so that no lane idles behind a row's end and what is open
 // in memory at a time is whole rows; the rows' sums of d_hidden * hidden go through shared memory, one number per unit, and are added up
-// in a fixed order.  135168 x 2048 back to back: 450 us, 6.2 TB/s (a warp per row with a conversion per byte: 506; a warp per row: 468; two rows
-// to a block: 509, sixteen: 450); one launch at 25088 x 1408 with a limit: 68 us (73, 77, 94, 70).  Held to 48 registers, a few of which
-// spill: with 64, 75 and 480 to 500 us, with 40, 80 and 482.
-// Back to back it is the board's power that bounds it (1 kW, 1.6 of 1.97 GHz), so instructions count: the sigmoid's quotient is the
-// approximate one, off by 2 steps of fp32, of which a step of bf16 is 65536 (IEEE: 500 us).
+// in a fixed order.  135168 x 2048 back to back: 445 us, 6.3 TB/s; one launch at 25088 x 1408 with a limit: 71 us.  Held to 48 registers, a few of
+// which spill: with 64, 454 and 71 us, with 76, 513 and 81.  (Tried with another quotient, which took 427 and 68 us: a warp per row 468 to
+// 506, two rows to a block 509, sixteen 450; limited 73 to 94 us.)
+// Back to back it is the board's power that bounds it (1 kW, 1.6 of 1.97 GHz), so instructions count.  The sigmoid's quotient is the IEEE one all
+// the same, as in mokb_swiglu_bwd: the approximate one rounds some gradients to the neighbouring bf16 number (6 of two million).
 constexpr int kRowsPerBlock = 8, kUnitsPerBlock = 8192;
 template <bool LIMIT>
 __global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
                     const float g0 = g4[b] * gs, u0 = u4[b] * us;
                     const float d = b & 1 ? bf16_hi(dh[2 * j + (b >> 1)]) : bf16_lo(dh[2 * j + (b >> 1)]);
                     const float g = LIMIT ? min_nan(g0, limit) : g0, up = LIMIT ? min_nan(max_nan(u0, -limit), limit) : u0;
-                    const float sig = __fdividef(0.25f, fmaf(0.25f, __expf(-g), 0.25f));
+                    const float sig = 1.0f / (1.0f + __expf(-g));
                     const float silu = g * sig;
                     h[b] = silu * up;
                     dg[b] = ((1.0f - silu) * sig + silu) * up * d;

@@ -1,4 +1,5 @@
-"""The backward pass of SwiGLU (whole, packed and quantising) at weights where 1 / w leaves fp32's range, and at rows without a weight."""
+"""The backward pass of SwiGLU (whole, packed and quantising) at weights where 1 / w leaves fp32's range, at rows without a weight, and
+the packed form's arithmetic against the whole one's."""
 import math
 
 import pytest
@@ -7,6 +8,15 @@ import torch
 from tests import plain_forms as P
 
 pytestmark = pytest.mark.gpu
+
+
+def whole_numbers(rows, cols, seed):
+    """bf16 values that packing holds exactly: whole numbers up to 127 times a power of two per block, 127 in every block."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    v = torch.randint(-127, 128, (rows, cols // 128, 128), generator=gen, device="cuda").float()
+    v[..., 0] = 127.0
+    v *= torch.exp2(torch.randint(-9, 1, (rows, cols // 128, 1), generator=gen, device="cuda").float())
+    return v.view(rows, cols).bfloat16()
 
 
 TINY = [1e-45, 1e-42, 1e-39, 2.0 ** -128, 2.0 ** -127, 2.0 ** -126, 1e-30, 0.5]
@@ -108,3 +118,19 @@ def test_a_row_without_a_weight_has_no_row_gradient():
         got = ops.swiglu_bwd_packed(*ops.pack_rows(gate), *ops.pack_rows(up), dh, limit, w)[3]
         assert (got[:7] == 0).all(), got
         assert torch.isfinite(got[7]) and got[7] > 0
+
+
+@pytest.mark.parametrize("limit", [None, 7.0, 0.25], ids=["free", "7", "quarter"])
+def test_packed_gradients_are_the_whole_forms_to_the_bit(limit):
+    """Of gate and up that packing holds exactly, d_gate and d_up are mokb_swiglu_bwd's: the same operations on the same numbers, none
+    of them in fewer bits."""
+    from mok import _C, ops
+    n, c = 2048, 1024
+    gate, up = whole_numbers(n, c, 3), whole_numbers(n, c, 4)
+    dh = torch.randn(n, c, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").bfloat16()
+    gp, upk = ops.pack_rows(gate), ops.pack_rows(up)
+    assert torch.equal(ops.unpack_rows(*gp), gate) and torch.equal(ops.unpack_rows(*upk), up)
+    got = ops.swiglu_bwd_packed(*gp, *upk, dh, limit)
+    want = _C.swiglu_bwd(gate, up, dh, limit)
+    assert torch.equal(got[0], want[0]), int((got[0] != want[0]).sum())
+    assert torch.equal(got[1], want[1]), int((got[1] != want[1]).sum())
