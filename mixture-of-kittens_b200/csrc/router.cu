@@ -54,6 +54,21 @@ template <bool BF16> __device__ __forceinline__ float load_one(const void* p, in
     return BF16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];
 }
 
+// This lane's part of a row in shared memory.
+template <int PER, bool VEC>
+__device__ __forceinline__ void load_shared(const float* row, int lane, float (&v)[PER]) {
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(row + expert_of<VEC>(i, lane));
+            v[i] = w.x; v[i + 1] = w.y; v[i + 2] = w.z; v[i + 3] = w.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] = row[expert_of<VEC>(i, lane)];
+    }
+}
+
 // This lane's logits of one row as they are; -inf beyond E.
 template <int PER, bool BF16, bool VEC>
 __device__ __forceinline__ void load_row(const RouteParams& p, int64_t row, int lane, float (&v)[PER]) {
@@ -126,6 +141,20 @@ template <bool SIGMOID>
 __device__ __forceinline__ float score_of(float l, float top, float inv_total) {
     return SIGMOID ? sigmoid(l) : l == -INFINITY ? 0.0f : exp2_approx((l - top) * kLog2E) * inv_total;
 }
+
+// The picks' shares of the sum of their scores (lane k: the k-th pick, l = -inf in the others and for closed ones) come from scores relative to
+// the largest pick's: exp(l - max), with sigmoid scores exp(l - c) / (1 + exp(l)) and c = min(max, 0).  So a row whose scores are all tiny still
+// has shares, and nothing is divided by a number that has lost its bits.  c stays above -641: logits below -744, whose score is 0 in 64 bits
+// too, are 0 here.
+template <bool SIGMOID>
+__device__ __forceinline__ float relative_score(float l, float max_l) {
+    if (!SIGMOID) return l == -INFINITY ? 0.0f : expf(l - max_l);
+    const float small = expf(-fabsf(l));
+    float r = l >= 0.0f ? 1.0f : small;
+    if (max_l < 0.0f) r = expf(l - fmaxf(max_l, -641.0f));      // (the same in every lane: max_l is the row's)
+    return r / (1.0f + small);
+}
+__device__ __forceinline__ float warp_max(float v) { return key_value(__reduce_max_sync(0xffffffffu, order_key(v))); }
 
 constexpr int index_bits(int per) { return per == 4 ? 7 : per == 8 ? 8 : per == 16 ? 9 : 10; }
 
@@ -270,10 +299,13 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
                 if (lane < p.K && l > -INFINITY) atomicAdd(&sm[mine], 1);
             }
         }
-        float s = lane < p.K ? score_of<SIGMOID>(l, top, inv_total) : 0.0f;
-        if (p.renormalize) {
+        float s;
+        if (p.renormalize) {          // (the first pick's logit is the largest unless a bias has picked)
+            s = relative_score<SIGMOID>(l, SIGMOID && p.bias ? warp_max(l) : __shfl_sync(0xffffffffu, l, 0));
             const float norm = warp_sum(s);
-            s = norm > 0.0f ? s / norm : 0.0f;
+            s = norm > 0.0f ? s / norm : 0.0f;          // (0: no pick is open)
+        } else {
+            s = score_of<SIGMOID>(l, top, inv_total);
         }
         if (lane < p.K) {
             p.top_experts[row * p.K + lane] = mine;
@@ -334,22 +366,24 @@ __global__ void __launch_bounds__(1024) route_reduce_kernel(const int32_t* part_
     }
 }
 
-// d s_k from d w_k: scale * d w_k, or with `renormalize` scale * (d w_k - sum_j share_j d w_j) / norm; plus d_score_sums on every
-// expert.  Then d l = s (d s - sum s d s) (softmax) or d s * s (1 - s) (sigmoid).
-// The picks' part of d s goes to the lanes that hold those experts through shared memory: a row of E numbers per warp that holds
-// d_score_sums (or zeros) between tokens.
+// The gradient of the logits has two parts.  The picks' own, worked out by the lane of a pick and handed through shared memory (a row of zeros
+// per warp between tokens) to the lane that holds its logit:
+//   renormalised   share_k (dw_k - sum_j share_j dw_j), with sigmoid scores times 1 - s_k    (dw: d_router_weights times scale)
+//   softmax        s_k dw_k                   sigmoid   s_k (1 - s_k) dw_k
+// and that of the scores: s_e (ds_e - dot) (softmax) or s_e (1 - s_e) ds_e (sigmoid) with ds = d_score_sums, which lies in shared memory once
+// per block, and dot = sum s ds (+ sum s_k dw_k where the weights are scores).  Without either the row's scores are not needed.
 template <int PER, bool BF16, bool VEC, bool SIGMOID>
 __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) route_bwd_kernel(const RouteParams p) {
     extern __shared__ __align__(16) float rows_sm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    float* const ds_sm = rows_sm + warp * PER * 32;
-    uint8_t* const tag_sm = reinterpret_cast<uint8_t*>(rows_sm + warps * PER * 32) + warp * PER * 32;      // who wrote an expert's number last
+    float* const part_sm = rows_sm + warp * PER * 32;
+    float* const sums_sm = rows_sm + warps * PER * 32;
+    uint8_t* const tag_sm = reinterpret_cast<uint8_t*>(sums_sm + PER * 32) + warp * PER * 32;      // who wrote an expert's number last
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int e = expert_of<VEC>(i, lane);
-        ds_sm[e] = p.d_score_sums && e < p.E ? __ldg(p.d_score_sums + e) : 0.0f;
-    }
-    __syncwarp();          // (a pick's number is read by the lane of the pick, not by the one that has filled it in)
+    for (int i = 0; i < PER; ++i) part_sm[expert_of<VEC>(i, lane)] = 0.0f;
+    const bool with_sums = p.d_score_sums != nullptr, with_scores = with_sums || (!SIGMOID && !p.renormalize);
+    for (int e = threadIdx.x; e < PER * 32; e += blockDim.x) sums_sm[e] = with_sums && e < p.E ? __ldg(p.d_score_sums + e) : 0.0f;
+    __syncthreads();
     const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
     int64_t row = static_cast<int64_t>(blockIdx.x) * warps + warp;
     float next[PER];
@@ -371,65 +405,75 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         const float dw = mine >= 0 ? next_dw * p.scale : 0.0f;
         const float l = mine >= 0 ? load_clean<BF16>(p, row, mine) : -INFINITY;
         if (row + step < p.T) fetch(row + step);
-        float top = 0.0f, inv_total = 1.0f;
-        if (!SIGMOID) {
-            top = v[0];
+        float top = 0.0f, inv_total = 1.0f, dot = 0.0f;
+        if (with_scores) {
+            if (!SIGMOID) {
+                top = v[0];
 #pragma unroll
-            for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
-            top = key_value(__reduce_max_sync(0xffffffffu, order_key(top)));
-        }
-        const float total = exponentials<PER, SIGMOID>(v, top);
-        if (!SIGMOID) {
-            inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
+                for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
+                top = warp_max(top);
+            }
+            const float total = exponentials<PER, SIGMOID>(v, top);
+            if (!SIGMOID) {
+                inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] *= inv_total;
+                for (int i = 0; i < PER; ++i) v[i] *= inv_total;
+            }
         }
-        const float s = score_of<SIGMOID>(l, top, inv_total);
-        float d = dw;
+        float part;
         if (p.renormalize) {
-            float norm = s, mean = s * dw;
+            const float r = relative_score<SIGMOID>(l, warp_max(l));
+            float norm = r, mean = r * dw;
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
                 norm += __shfl_xor_sync(0xffffffffu, norm, o);
                 mean += __shfl_xor_sync(0xffffffffu, mean, o);
             }
-            const float inv = norm > 0.0f ? 1.0f / norm : 0.0f;
-            d = (dw - mean * inv) * inv;
+            const float inv = norm > 0.0f ? 1.0f / norm : 0.0f;          // (norm is 1/2 or more where a pick is open)
+            part = r * inv * (dw - mean * inv);
+            if (SIGMOID) part *= 1.0f - sigmoid(l);
+        } else {
+            const float s = score_of<SIGMOID>(l, top, inv_total);
+            part = SIGMOID ? s * (1.0f - s) * dw : s * dw;
+            if (!SIGMOID) dot = part;                // (added up below, with the scores' own)
         }
-        float kept = 0.0f;
-        if (mine >= 0) {
-            kept = ds_sm[mine];
-            tag_sm[mine] = static_cast<uint8_t>(lane);
-        }
+        if (mine >= 0) tag_sm[mine] = static_cast<uint8_t>(lane);
         __syncwarp();
-        if (mine >= 0) ds_sm[mine] = kept + d;
+        if (mine >= 0) part_sm[mine] = part;
         if (__any_sync(0xffffffffu, mine >= 0 && tag_sm[mine] != lane)) {
             // a caller's list that names an expert twice: one after the other, in the list's order
-            if (mine >= 0) ds_sm[mine] = kept;
+            if (mine >= 0) part_sm[mine] = 0.0f;
             __syncwarp();
             for (int k = 0; k < p.K; ++k) {
-                if (lane == k && mine >= 0) ds_sm[mine] += d;
+                if (lane == k && mine >= 0) part_sm[mine] += part;
                 __syncwarp();
             }
         }
         __syncwarp();
-        float ds[PER];
+        if (with_scores) {
+            float ds[PER];
+            load_shared<PER, VEC>(sums_sm, lane, ds);
+            if (SIGMOID) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) ds[i] = ds_sm[expert_of<VEC>(i, lane)];
-        __syncwarp();
-        if (mine >= 0) ds_sm[mine] = kept;
-        __syncwarp();
-        if (SIGMOID) {
+                for (int i = 0; i < PER; ++i) v[i] = ds[i] * v[i] * (1.0f - v[i]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] = ds[i] * v[i] * (1.0f - v[i]);
+                for (int i = 0; i < PER; ++i) dot += v[i] * ds[i];
+                dot = warp_sum(dot);
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[i] *= ds[i] - dot;
+            }
         } else {
-            float dot = 0.0f;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) dot += v[i] * ds[i];
-            dot = warp_sum(dot);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) v[i] *= ds[i] - dot;
+            for (int i = 0; i < PER; ++i) v[i] = 0.0f;
         }
+        float own[PER];
+        load_shared<PER, VEC>(part_sm, lane, own);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) v[i] += own[i];
+        __syncwarp();
+        if (mine >= 0) part_sm[mine] = 0.0f;
+        __syncwarp();
         const int64_t base = row * p.E;
         if (VEC) {
 #pragma unroll
@@ -460,7 +504,8 @@ int route_blocks(int64_t T, int E) {
 template <int PER, bool BF16, bool VEC, bool SIGMOID>
 int launch_route(const RouteParams& p, bool backward, cudaStream_t stream) {
     const int blocks = route_blocks(p.T, PER * 32);
-    if (backward) route_bwd_kernel<PER, BF16, VEC, SIGMOID><<<blocks, route_threads(PER), route_threads(PER) * PER * 5, stream>>>(p);
+    if (backward)      // a row of numbers and tags per warp, d_score_sums once
+        route_bwd_kernel<PER, BF16, VEC, SIGMOID><<<blocks, route_threads(PER), (route_threads(PER) * 5 + 128) * PER, stream>>>(p);
     else route_kernel<PER, BF16, VEC, SIGMOID><<<blocks, route_threads(PER), p.part_count ? 8u * p.E : 0u, stream>>>(p);
     MOKB_CUDA(cudaGetLastError());
     note_launch();

@@ -25,3 +25,41 @@ def test_a_warps_first_row_has_the_score_sums_gradient(score, renorm, E, K):
     first = check_backward(cfg, logits, r)
     for _ in range(10):
         assert torch.equal(check_backward(cfg, logits, r), first)
+
+
+def spread_logits(T, E, far, seed, step=0.25):
+    """fp32 logits on multiples of `step`, so that differences of two are exact, from 0 down to -far."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    l = -torch.randint(0, int(far / step) + 1, (T, E), generator=gen, device="cuda").float() * step
+    l[:, 0] = 0.0
+    return l
+
+
+@pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("level", [-80.0, -90.0, -100.0, -110.0, -300.0, -600.0])
+def test_shares_of_sigmoid_scores_far_below_zero(level, dtype, bias):
+    """Renormalised weights are shares of the scores' sum however small the scores are: the token keeps its experts, and the gradient
+    its slope.  A share: two exps, a quotient each, a product (12), a sum of K (5), a quotient (1), `scale` (1)."""
+    from mok import functional as F
+    E, K = 32, 6
+    logits = (level + spread_logits(300, E, 12.0, seed=3, step=0.5)).to(dtype)      # (halves, exact in bf16 only near zero: as rounded)
+    b = torch.zeros(E, device="cuda")
+    b[::4] = 0.25
+    b = b if bias else None
+    cfg = F.MoKRouterConfig(topk=K, score="sigmoid", scale=2.5)
+    r = F.route(cfg, logits, b)
+    picked, weights, _, _, _, _ = P.route(logits, K, "sigmoid", b, True, 2.5)
+    assert torch.equal(r.top_experts, picked)
+    assert ((r.router_weights.double() - weights).abs() <= 20 * U * weights + 2.0 ** -149).all()
+    assert ((r.router_weights.double().sum(1) - 2.5).abs() <= 2.5 * (20 + K) * U).all()
+    dw = torch.randn(300, K, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    d = F.route_backward(cfg, logits, r, dw)
+    want = P.route_bwd(logits, picked, dw, None, "sigmoid", True, 2.5)
+    # share * (dw - mean): dw and the mean, each off by 30 roundings of itself, the share by 20
+    share = weights / 2.5
+    terms = 2.5 * share * (dw.double().abs() + (share * dw.double().abs()).sum(1, keepdim=True))
+    room = torch.zeros_like(want).scatter_(1, picked, 64 * U * terms) + 2.0 ** -149
+    if dtype == torch.bfloat16:
+        room = room + P.U16 * (want.abs() + room)
+    assert ((d.double() - want).abs() <= room).all()
