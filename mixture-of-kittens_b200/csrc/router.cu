@@ -115,12 +115,19 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 constexpr uint32_t kClosedKey = 0x007fffffu;          // order_key(-inf)
-constexpr float kLog2E = 1.4426950408889634f;
-__device__ __forceinline__ float exp2_approx(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
-__device__ __forceinline__ float sigmoid(float l) { return __fdividef(1.0f, 1.0f + exp2_approx(-kLog2E * l)); }      // (-inf: 0)
+// Scores that leave the kernel come from expf and IEEE quotients and reciprocals: an approximate exp's error grows with its argument (58
+// half-steps of fp32 for a softmax logit 80 below the largest), and an approximate quotient of 1 by 1 + exp(-l) is 0 from logits of -87 on,
+// where fp32 holds scores down to -103.  (IEEE quotients in place of the reciprocals below, whose argument is between 1 and 2: 1 to 3 us
+// more on 32768 x 128; approximate reciprocals: 1 to 1.5 us less, 3.5 on 16384 x 512.)
+__device__ __forceinline__ float sigmoid(float l) {      // (-inf: 0)
+    const float small = expf(-fabsf(l));
+    return (l >= 0.0f ? 1.0f : small) * __frcp_rn(1.0f + small);
+}
+// For the order of the picks alone, which is settled by better sums wherever this could decide it.
+__device__ __forceinline__ float sigmoid_for_order(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
 
 // exp(l - top) of a row's logits, in place, and their sum (SIGMOID: the scores themselves).  Closed ones give 0; a row that is closed as a
-// whole has top = -inf.  The exponent is one rounding of a product and one of a sum off: |top| + |l - top| half units.
+// whole has top = -inf.
 template <int PER, bool SIGMOID>
 __device__ __forceinline__ float exponentials(float (&v)[PER], float top) {
     if (SIGMOID) {
@@ -132,14 +139,14 @@ __device__ __forceinline__ float exponentials(float (&v)[PER], float top) {
     const float at = top == -INFINITY ? 0.0f : top;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        v[i] = exp2_approx((v[i] - at) * kLog2E);
+        v[i] = expf(v[i] - at);
         total += v[i];
     }
     return warp_sum(total);
 }
 template <bool SIGMOID>
-__device__ __forceinline__ float score_of(float l, float top, float inv_total) {
-    return SIGMOID ? sigmoid(l) : l == -INFINITY ? 0.0f : exp2_approx((l - top) * kLog2E) * inv_total;
+__device__ __forceinline__ float score_of(float l, float top, float total) {
+    return SIGMOID ? sigmoid(l) : l == -INFINITY ? 0.0f : expf(l - top) / total;      // (a logit that is open has a total of 1 or more)
 }
 
 // The picks' shares of the sum of their scores (lane k: the k-th pick, l = -inf in the others and for closed ones) come from scores relative to
@@ -152,7 +159,7 @@ __device__ __forceinline__ float relative_score(float l, float max_l) {
     const float small = expf(-fabsf(l));
     float r = l >= 0.0f ? 1.0f : small;
     if (max_l < 0.0f) r = expf(l - fmaxf(max_l, -641.0f));      // (the same in every lane: max_l is the row's)
-    return r / (1.0f + small);
+    return r * __frcp_rn(1.0f + small);
 }
 __device__ __forceinline__ float warp_max(float v) { return key_value(__reduce_max_sync(0xffffffffu, order_key(v))); }
 
@@ -242,10 +249,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         for (int i = 0; i < PER; ++i) {
             const int e = expert_of<VEC>(i, lane);
             float order = v[i];
-            if (SIGMOID && p.bias) {
-                v[i] = sigmoid(order);       // (0 where closed)
-                if (order > -INFINITY && e < p.E) order = clean(v[i] + __ldg(p.bias + e));      // (a NaN's key could be none)
-            }
+            if (SIGMOID && p.bias && order > -INFINITY && e < p.E) order = clean(sigmoid_for_order(order) + __ldg(p.bias + e));      // (a NaN's key could be none)
             key[i] = e >= p.E ? 0u : (order_key(order) & ~kIndex) | (kIndex - static_cast<uint32_t>(e));
         }
         constexpr bool kExact = BF16 && !SIGMOID;      // (a bf16 logit's key loses nothing to the index)
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         int mine = static_cast<int>(kIndex - (mine_key & kIndex));      // lane k: the k-th pick
         float l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
         if (SIGMOID && p.bias) {
-            // The picks' sums as they are, and the largest that one which is left out can be.  s in 32 bits: an exp (off by some 2 + 1.2 |l|
+            // The picks' sums as they are, and the largest that one which is left out can be.  s of a key: an exp (off by some 2 + 1.2 |l|
             // units in the last place; s (1 - s) <= 1/4 and |l| s (1 - s) < 0.23 of that), a sum and a quotient: below 3e-7.  s + bias and the
             // 32-bit form of the exact sum are rounded once each.  Neighbours that are more than 1e-6 (1 + |s + bias|) apart are in order.
             const float hi = l > -INFINITY ? clean(sigmoid(l) + __ldg(p.bias + mine)) : -INFINITY;
@@ -288,14 +292,14 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
                 l = lane < p.K ? load_clean<BF16>(p, row, mine) : -INFINITY;
             }
         }
-        float inv_total = 1.0f, top = 0.0f;
+        float total = 1.0f, top = 0.0f;
         if (!SIGMOID) top = __shfl_sync(0xffffffffu, l, 0);          // the first pick has the largest logit
         if (balance || (!SIGMOID && !p.renormalize)) {
-            const float total = SIGMOID && p.bias ? 1.0f : exponentials<PER, SIGMOID>(v, top);
-            if (!SIGMOID) inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
+            total = exponentials<PER, SIGMOID>(v, top);
             if (balance) {
+                const float inv_total = SIGMOID ? 1.0f : total > 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
-                for (int i = 0; i < PER; ++i) acc[i] += v[i] * inv_total;
+                for (int i = 0; i < PER; ++i) acc[i] += SIGMOID ? v[i] : v[i] * inv_total;
                 if (lane < p.K && l > -INFINITY) atomicAdd(&sm[mine], 1);
             }
         }
@@ -305,7 +309,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
             const float norm = warp_sum(s);
             s = norm > 0.0f ? s / norm : 0.0f;          // (0: no pick is open)
         } else {
-            s = score_of<SIGMOID>(l, top, inv_total);
+            s = score_of<SIGMOID>(l, top, total);
         }
         if (lane < p.K) {
             p.top_experts[row * p.K + lane] = mine;
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         const float dw = mine >= 0 ? next_dw * p.scale : 0.0f;
         const float l = mine >= 0 ? load_clean<BF16>(p, row, mine) : -INFINITY;
         if (row + step < p.T) fetch(row + step);
-        float top = 0.0f, inv_total = 1.0f, dot = 0.0f;
+        float top = 0.0f, total = 1.0f, dot = 0.0f;
         if (with_scores) {
             if (!SIGMOID) {
                 top = v[0];
@@ -413,9 +417,9 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
                 for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
                 top = warp_max(top);
             }
-            const float total = exponentials<PER, SIGMOID>(v, top);
+            total = exponentials<PER, SIGMOID>(v, top);
             if (!SIGMOID) {
-                inv_total = total > 0.0f ? __fdividef(1.0f, total) : 0.0f;
+                const float inv_total = total > 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) v[i] *= inv_total;
             }
@@ -433,7 +437,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
             part = r * inv * (dw - mean * inv);
             if (SIGMOID) part *= 1.0f - sigmoid(l);
         } else {
-            const float s = score_of<SIGMOID>(l, top, inv_total);
+            const float s = score_of<SIGMOID>(l, top, total);
             part = SIGMOID ? s * (1.0f - s) * dw : s * dw;
             if (!SIGMOID) dot = part;                // (added up below, with the scores' own)
         }

@@ -35,6 +35,35 @@ def spread_logits(T, E, far, seed, step=0.25):
     return l
 
 
+@pytest.mark.parametrize("renorm", [True, False], ids=["share", "score"])
+def test_softmax_far_below_the_largest_logit(renorm):
+    """The error of a score does not grow with its distance from the row's largest: an exp (4 half-steps), a sum of at most E of them
+    (4 and 7 additions for 8 experts: a lane's four slots, a tree of five over the warp, 9 at most), a quotient, `scale` (1): 16."""
+    from mok import functional as F
+    E = K = 8
+    logits = spread_logits(4000, E, 80.0, seed=1)
+    r = F.route(F.MoKRouterConfig(topk=K, renormalize=renorm), logits, balance=True)
+    picked, weights, _, sums, s, _ = P.route(logits, K, "softmax", None, renorm)
+    assert torch.equal(r.top_experts, picked)
+    off = (r.router_weights.double() - weights).abs() / (U * weights)
+    assert off.max() <= 16, off.max()
+    # a warp adds at most ceil(T / warps) rows, a block its warps, the reduction its blocks: below 200 additions of positive numbers
+    assert ((r.score_sums.double() - sums).abs() <= (16 + 200) * U * sums).all()
+
+
+@pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
+def test_sigmoid_over_its_range(bias):
+    """Scores of logits from -100 to 100, fp32's subnormal numbers included: an exp, a sum, a quotient, a product: 8 half-steps, and
+    half a step of the smallest number."""
+    from mok import functional as F
+    E = K = 16
+    logits = spread_logits(2000, E, 200.0, seed=2) + 100.0
+    b = torch.zeros(E, device="cuda") if bias else None
+    r = F.route(F.MoKRouterConfig(topk=K, score="sigmoid", renormalize=False), logits, b)
+    want = torch.sigmoid(logits.double()).gather(1, r.top_experts)
+    assert ((r.router_weights.double() - want).abs() <= 8 * U * want + 2.0 ** -149).all()
+
+
 @pytest.mark.parametrize("bias", [False, True], ids=["plain", "bias"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 @pytest.mark.parametrize("level", [-80.0, -90.0, -100.0, -110.0, -300.0, -600.0])
