@@ -123,6 +123,11 @@ __device__ __forceinline__ float sigmoid(float l) {      // (-inf: 0)
     const float small = expf(-fabsf(l));
     return (l >= 0.0f ? 1.0f : small) * __frcp_rn(1.0f + small);
 }
+// s (1 - s): of s near 1 the difference from 1 would be what rounding has left of it.
+__device__ __forceinline__ float sigmoid_slope(float l) {      // (-inf: 0)
+    const float small = expf(-fabsf(l)), q = __frcp_rn(1.0f + small);
+    return small * q * q;
+}
 // For the order of the picks alone, which is settled by better sums wherever this could decide it.
 __device__ __forceinline__ float sigmoid_for_order(float l) { return __fdividef(1.0f, 1.0f + __expf(-l)); }
 
@@ -410,15 +415,16 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         const float l = mine >= 0 ? load_clean<BF16>(p, row, mine) : -INFINITY;
         if (row + step < p.T) fetch(row + step);
         float top = 0.0f, total = 1.0f, dot = 0.0f;
-        if (with_scores) {
-            if (!SIGMOID) {
+        if (with_scores) {          // v: what d_score_sums is multiplied by, the scores or the sigmoid's slope
+            if (SIGMOID) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) v[i] = sigmoid_slope(v[i]);
+            } else {
                 top = v[0];
 #pragma unroll
                 for (int i = 1; i < PER; ++i) top = fmaxf(top, v[i]);
                 top = warp_max(top);
-            }
-            total = exponentials<PER, SIGMOID>(v, top);
-            if (!SIGMOID) {
+                total = exponentials<PER, false>(v, top);
                 const float inv_total = total > 0.0f ? 1.0f / total : 0.0f;
 #pragma unroll
                 for (int i = 0; i < PER; ++i) v[i] *= inv_total;
@@ -435,10 +441,9 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
             }
             const float inv = norm > 0.0f ? 1.0f / norm : 0.0f;          // (norm is 1/2 or more where a pick is open)
             part = r * inv * (dw - mean * inv);
-            if (SIGMOID) part *= 1.0f - sigmoid(l);
+            if (SIGMOID) part *= sigmoid(-l);          // 1 - s
         } else {
-            const float s = score_of<SIGMOID>(l, top, total);
-            part = SIGMOID ? s * (1.0f - s) * dw : s * dw;
+            part = (SIGMOID ? sigmoid_slope(l) : score_of<false>(l, top, total)) * dw;
             if (!SIGMOID) dot = part;                // (added up below, with the scores' own)
         }
         if (mine >= 0) tag_sm[mine] = static_cast<uint8_t>(lane);
@@ -459,7 +464,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
             load_shared<PER, VEC>(sums_sm, lane, ds);
             if (SIGMOID) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) v[i] = ds[i] * v[i] * (1.0f - v[i]);
+                for (int i = 0; i < PER; ++i) v[i] *= ds[i];
             } else {
 #pragma unroll
                 for (int i = 0; i < PER; ++i) dot += v[i] * ds[i];

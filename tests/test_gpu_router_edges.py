@@ -92,3 +92,61 @@ def test_shares_of_sigmoid_scores_far_below_zero(level, dtype, bias):
     if dtype == torch.bfloat16:
         room = room + P.U16 * (want.abs() + room)
     assert ((d.double() - want).abs() <= room).all()
+
+
+@pytest.mark.parametrize("renorm", [True, False], ids=["share", "score"])
+def test_sigmoid_gradient_near_one(renorm):
+    """Logits up to 40: 1 - s is a small number of its own, not what is left of 1 after s is rounded."""
+    from mok import functional as F
+    E, K = 24, 4
+    logits = spread_logits(500, E, 35.0, seed=5) + 40.0
+    cfg = F.MoKRouterConfig(topk=K, score="sigmoid", renormalize=renorm)
+    r = F.route(cfg, logits)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    dw, ds = torch.randn(500, K, generator=gen, device="cuda"), torch.randn(E, generator=gen, device="cuda")
+    d = F.route_backward(cfg, logits, r, dw, ds)
+    l = logits.double()
+    s, c = torch.sigmoid(l), torch.sigmoid(-l)
+    chosen = s.gather(1, r.top_experts)
+    g = dw.double()
+    if renorm:
+        share = chosen / chosen.sum(1, keepdim=True)
+        part, size = share * (g - (share * g).sum(1, keepdim=True)), share * (g.abs() + (share * g.abs()).sum(1, keepdim=True))
+    else:
+        part, size = chosen * g, (chosen * g).abs()
+    want = (s * ds.double()).scatter_add(1, r.top_experts, part) * c
+    room = (s * ds.double().abs()).scatter_add(1, r.top_experts, size) * c
+    assert ((d.double() - want).abs() <= 64 * U * room).all()
+
+
+@pytest.mark.parametrize("E,dtype", [(128, torch.float32), (127, torch.bfloat16), (256, torch.bfloat16), (512, torch.float32), (1000, torch.bfloat16), (1024, torch.float32)],
+                         ids=lambda v: str(v).replace("torch.", ""))
+@pytest.mark.parametrize("score,bias,renorm", [("softmax", False, True), ("softmax", False, False), ("sigmoid", False, True), ("sigmoid", True, True),
+                                               ("sigmoid", True, False)])
+def test_several_rows_per_warp(score, bias, renorm, E, dtype):
+    """More rows than the grid has warps: every warp carries its prefetched row, its sums and its shared-memory row on to the next.  All
+    values against 64 bits, with d_score_sums and no zero among d_weights; the load figures to what their additions allow."""
+    from mok import functional as F
+    T = 15013
+    logits = logits_of(T, E, dtype, seed=E)
+    b = torch.randn(E, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda") * 0.2 if bias else None
+    cfg = F.MoKRouterConfig(topk=5, score=score, renormalize=renorm, scale=1.5)
+    r = check_forward(cfg, logits, b)
+    check_backward(cfg, logits, r)
+    # score_sums: a score (its own sum of E / 32 terms a lane and the warp's five steps, 24 more), then positive numbers added: at most
+    # 40 rows of a warp (15013 over 148 SMs of three blocks of four warps: 9), 8 warps, 8 blocks a thread of the reduction, 40 more
+    _, _, _, sums, _, _ = P.route(logits, 5, score, b, renorm, 1.5)
+    rough = (E // 32 + 32 + 40 + 8 + 8 + 40) * U
+    assert ((r.score_sums.double() - sums).abs() <= rough * sums).all()
+
+
+def test_long_batches_of_near_ties():
+    """Biased sums a few fp32 steps apart, 120000 rows: every pick is that of the 64-bit sums rounded to 32 bits."""
+    from mok import functional as F
+    E, K, T = 64, 6, 120000
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    s = 0.6 + torch.randint(-8, 9, (T, E), generator=gen, device="cuda").double() * 2.0 ** -25
+    logits = torch.log(s / (1 - s)).float()
+    bias = torch.randint(0, 3, (E,), generator=gen, device="cuda").float() * 2.0 ** -24
+    r = F.route(F.MoKRouterConfig(topk=K, score="sigmoid"), logits, bias)
+    assert torch.equal(r.top_experts, P.route(logits, K, "sigmoid", bias)[0])
