@@ -535,8 +535,8 @@ int mokb_few_tokens_fwd(const mokb_few_tokens_args* args, void* stream);
  *   MOKB_SCORE_SOFTMAX  s = softmax(logits), the largest logits are picked
  *   MOKB_SCORE_SIGMOID  s = 1 / (1 + exp(-logits)), the largest s + bias are picked (bias [num_experts], optional; worked out in
  *                       64 bits and compared as 32-bit numbers)
- *   weights: scale * s of the picks, with `renormalize` divided by their sum (also where that sum is below fp32's range; sigmoid scores
- *   of logits below -744, which are 0 in 64 bits, are 0)
+ *   weights: scale * s of the picks, with `renormalize` divided by their sum (also where that sum is below fp32's range; where
+ *   all picks' logits are below -745, and their sigmoid is 0 in 64 bits too, the weights are 0)
  * Picks come in falling order, ties go to the lowest index; experts whose logit is -inf or NaN are closed: s = 0, picked only
  * when nothing else is left, lowest index first, with weight 0.  +inf counts as the largest finite number.
  * Load figures (optional, together; scratch: mokb_route_scratch_bytes()): tokens_per_expert [num_experts] int32, picks of open

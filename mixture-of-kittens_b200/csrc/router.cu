@@ -156,14 +156,13 @@ __device__ __forceinline__ float score_of(float l, float top, float total) {
 
 // The picks' shares of the sum of their scores (lane k: the k-th pick, l = -inf in the others and for closed ones) come from scores relative to
 // the largest pick's: exp(l - max), with sigmoid scores exp(l - c) / (1 + exp(l)) and c = min(max, 0).  So a row whose scores are all tiny still
-// has shares, and nothing is divided by a number that has lost its bits.  c stays above -641: logits below -744, whose score is 0 in 64 bits
-// too, are 0 here.
+// has shares, and their sum is 1/2 or more.  A row whose largest pick lies below -745, where sigmoid is 0 in 64 bits too, has none.
 template <bool SIGMOID>
 __device__ __forceinline__ float relative_score(float l, float max_l) {
     if (!SIGMOID) return l == -INFINITY ? 0.0f : expf(l - max_l);
     const float small = expf(-fabsf(l));
     float r = l >= 0.0f ? 1.0f : small;
-    if (max_l < 0.0f) r = expf(l - fmaxf(max_l, -641.0f));      // (the same in every lane: max_l is the row's)
+    if (max_l < 0.0f) r = max_l < -745.0f ? 0.0f : expf(l - max_l);      // (the same in every lane: max_l is the row's)
     return r * __frcp_rn(1.0f + small);
 }
 __device__ __forceinline__ float warp_max(float v) { return key_value(__reduce_max_sync(0xffffffffu, order_key(v))); }

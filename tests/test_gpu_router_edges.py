@@ -94,6 +94,29 @@ def test_shares_of_sigmoid_scores_far_below_zero(level, dtype, bias):
     assert ((d.double() - want).abs() <= room).all()
 
 
+@pytest.mark.parametrize("level", [-640.0, -700.0, -720.0, -735.0, -742.0, -744.5, -746.0, -800.0, -1e30])
+def test_shares_at_the_end_of_the_sigmoids_range(level):
+    """Rows whose largest pick's score is just inside 64 bits' range (exp(-745)) have shares and a gradient, rows beyond have none; never
+    a NaN or an infinity.  One share per distance from the largest: the expected ones are exp of it, over their sum."""
+    from mok import functional as F
+    E = K = 4
+    below = torch.tensor([0.0, 0.25, 0.5, 0.0], device="cuda")
+    logits = (level - below).expand(8, E).contiguous()
+    cfg = F.MoKRouterConfig(topk=K, score="sigmoid")
+    r = F.route(cfg, logits, balance=True)
+    dw = torch.randn(8, K, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda")
+    d = F.route_backward(cfg, logits, r, dw, torch.ones(E, device="cuda"))
+    assert torch.isfinite(r.router_weights).all() and torch.isfinite(d).all()
+    if level < -745:
+        assert (r.router_weights == 0).all() and (d == 0).all()
+        return
+    share = torch.softmax(logits.double(), 1).gather(1, r.top_experts)
+    assert ((r.router_weights.double() - share).abs() <= 20 * U * share).all()
+    want = share * (dw.double() - (share * dw.double()).sum(1, keepdim=True))
+    size = share * (dw.double().abs() + (share * dw.double().abs()).sum(1, keepdim=True))
+    assert ((d.double().gather(1, r.top_experts) - want).abs() <= 64 * U * size).all()
+
+
 @pytest.mark.parametrize("renorm", [True, False], ids=["share", "score"])
 def test_sigmoid_gradient_near_one(renorm):
     """Logits up to 40: 1 - s is a small number of its own, not what is left of 1 after s is rounded."""
