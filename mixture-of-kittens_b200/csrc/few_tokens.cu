@@ -31,6 +31,10 @@
 // Three stages in the ring instead of six cost 4 %; units of 64 columns instead of 128 nothing up to 200 tokens, 45 % at 511 (their experts'
 // weights are then read twice).
 //
+// hidden is rounded to bf16 (MXFP8: E4M3) between the products: both operands of a tcgen05 product have the weights' type, and the layer's own
+// forward keeps it so.  Against 64 bits y is then off by 0.0023 of itself (root mean square) where a product of unrounded hidden would leave y's
+// own rounding, 0.0017; hidden as two bf16 parts would be nearer, for twice the narrow operand.
+//
 //   warp 0     TMA producer: weights (two 128-row boxes of 128 bytes per stage) and, MXFP8, their scale tiles
 //   warp 1     MMA issuer
 //   warps 2-9  epilogue
@@ -838,6 +842,9 @@ extern "C" int mokb_few_tokens_fwd(const mokb_few_tokens_args* a, void* stream_)
         dn.scale1 = dn.scale0;
     }
     MOKB_TRY(allow_shared_memory());
+    // The order of the four launches is part of their synchronisation: gate/up may trigger down only after it has seen the plan's end, so down
+    // and sum read the plan ahead of their own wait.  A launch between them, or a plan that is itself launched programmatically, would
+    // take that away.
     // few routes: fewer threads to start and to wait for
     const int plan_threads = p.T * p.K <= kPlanThreadsSmall && p.E <= 2 * kPlanThreadsSmall ? kPlanThreadsSmall : kPlanThreads;
     const int pieces = p.T * ((H + 1023) / 1024), quant_blocks = mx ? (pieces + plan_threads / 32 - 1) / (plan_threads / 32) : 0;

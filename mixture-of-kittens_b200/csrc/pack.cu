@@ -123,14 +123,14 @@ __device__ __forceinline__ float max_nan(float a, float b) { float r; asm("max.N
 
 // A block takes up to eight consecutive rows, its threads their units in order, so that no lane idles behind a row's end and what is open
 // in memory at a time is whole rows; the rows' sums of d_hidden * hidden go through shared memory, one number per unit, and are added up
-// in a fixed order.  135168 x 2048 back to back: 445 us, 6.3 TB/s; one launch at 25088 x 1408 with a limit: 71 us.  Held to 48 registers, a few of
-// which spill: with 64, 454 and 71 us, with 76, 513 and 81.  (Tried with another quotient, which took 427 and 68 us: a warp per row 468 to
-// 506, two rows to a block 509, sixteen 450; limited 73 to 94 us.)
+// in a fixed order.  135168 x 2048 back to back for a second: 467 us, 6.0 TB/s; 25088 x 1408 with a limit: 71 us.  64 registers, none spilled: held to
+// 48, of which a few spill, 477 and 71 us (one pass of pack, pack and this: 10 us more), with 76, 513 and 81.
+// (Tried with an approximate quotient, which took 430 and 67 us: a warp per row 468 to 506, two rows to a block 509, sixteen 450; limited 73 to 94.)
 // Back to back it is the board's power that bounds it (1 kW, 1.6 of 1.97 GHz), so instructions count.  The sigmoid's quotient is the IEEE one all
 // the same, as in mokb_swiglu_bwd: the approximate one rounds some gradients to the neighbouring bf16 number (6 of two million).
 constexpr int kRowsPerBlock = 8, kUnitsPerBlock = 8192;
 template <bool LIMIT>
-__global__ void __launch_bounds__(256, 5) swiglu_bwd_packed_kernel(
+__global__ void __launch_bounds__(256, 4) swiglu_bwd_packed_kernel(
     const int8_t* __restrict__ gate_q, const float* __restrict__ gate_sc, const int8_t* __restrict__ up_q, const float* __restrict__ up_sc,
     const __nv_bfloat16* __restrict__ d_hidden, __nv_bfloat16* __restrict__ d_gate, __nv_bfloat16* __restrict__ d_up,
     __nv_bfloat16* __restrict__ hidden, const float* __restrict__ row_scale, float* __restrict__ row_grad,
