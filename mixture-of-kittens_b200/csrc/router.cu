@@ -17,12 +17,13 @@
 // evaluated: the order is that of the sums worked out in 64 bits and rounded to 32.  They too are first picked by such keys; then the picks'
 // own sums in 32 bits, and the most that the next key can stand for, say whether that was the order, and the row is done again in 64 where
 // neighbours are nearer than the error of that.  (Asking the keys themselves, short of seven bits and more, sends 6 % of the rows there at
-// 128 experts: 28 us instead of 26; at 512 experts 57 instead of 39.)
+// 128 experts: 28 us where this took 26; at 512 experts 57 where it took 39.)
 // (16384 x 256, 8 picks: 28 us looking through all keys for every pick, 19 with keys and indices apart.)
 //
-// Bound by instruction issue at long micro-batches (60 to 77 % of the cycles issue, memory at a tenth of its rate).  Graph replays back to back:
-// 16384 x 256 in fp32, 8 picks: 11.8 us forward, 17.2 with the load figures, 8.7 backward; 32768 x 128 with a bias: 21.6, 26 and 10.3; 16384 x 512
-// with a bias: 34, 39 and 10.4.  The logits alone take 2.6 to 5.1 us.
+// Bound by instructions at long micro-batches: of a row of 256 logits 690 warp instructions in the forward pass with the load figures and 420 in
+// the backward pass, of 128 with a bias 680 and 320; 63 to 76 % of the cycles issue, memory is at a tenth to a third of its rate.  Graph replays back
+// to back: 16384 x 256 in fp32, softmax, 8 picks: 11.5 us forward, 17.8 with the load figures, 6.3 backward, 9.6 with score sums; 32768 x 128 with a
+// bias: 23.4, 30.0, 10.6 and 13.0; 16384 x 512 with a bias: 36.5, 45.8, 9.3 and 13.2.  The logits alone take 2.6 to 5.1 us.
 #include <float.h>
 
 #include "common.cuh"
@@ -115,17 +116,22 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 constexpr uint32_t kClosedKey = 0x007fffffu;          // order_key(-inf)
-// Scores that leave the kernel come from expf and IEEE quotients and reciprocals: an approximate exp's error grows with its argument (58
-// half-steps of fp32 for a softmax logit 80 below the largest), and an approximate quotient of 1 by 1 + exp(-l) is 0 from logits of -87 on,
-// where fp32 holds scores down to -103.  (IEEE quotients in place of the reciprocals below, whose argument is between 1 and 2: 1 to 3 us
-// more on 32768 x 128; approximate reciprocals: 1 to 1.5 us less, 3.5 on 16384 x 512.)
+// Scores that leave the kernel come from expf: an approximate exp's error grows with its argument (58 half-steps of fp32 for a softmax logit 80
+// below the largest).  Quotients that make a weight are IEEE ones.  The denominator of a sigmoid, 1 + exp(-|l|), is between 1 and 2: its
+// reciprocal is the IEEE one for the picks, and for all of a row's experts (load figures and the gradient of the score sums, where dozens
+// of roundings follow) the approximate one, off by two units in the last place at most.  With the IEEE one there too: 30.8 instead of
+// 30.0 us (32768 x 128, bias, figures) and 48.7 instead of 45.8 (16384 x 512), backward with score sums 14.2 and 17.0 instead of 13.0 and 13.2.
+template <bool MANY>
+__device__ __forceinline__ float reciprocal(float d) { return MANY ? __fdividef(1.0f, d) : __frcp_rn(d); }
+template <bool MANY>
 __device__ __forceinline__ float sigmoid(float l) {      // (-inf: 0)
     const float small = expf(-fabsf(l));
-    return (l >= 0.0f ? 1.0f : small) * __frcp_rn(1.0f + small);
+    return (l >= 0.0f ? 1.0f : small) * reciprocal<MANY>(1.0f + small);
 }
 // s (1 - s): of s near 1 the difference from 1 would be what rounding has left of it.
+template <bool MANY>
 __device__ __forceinline__ float sigmoid_slope(float l) {      // (-inf: 0)
-    const float small = expf(-fabsf(l)), q = __frcp_rn(1.0f + small);
+    const float small = expf(-fabsf(l)), q = reciprocal<MANY>(1.0f + small);
     return small * q * q;
 }
 // For the order of the picks alone, which is settled by better sums wherever this could decide it.
@@ -137,7 +143,7 @@ template <int PER, bool SIGMOID>
 __device__ __forceinline__ float exponentials(float (&v)[PER], float top) {
     if (SIGMOID) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = sigmoid(v[i]);
+        for (int i = 0; i < PER; ++i) v[i] = sigmoid<true>(v[i]);
         return 1.0f;
     }
     float total = 0.0f;
@@ -151,7 +157,7 @@ __device__ __forceinline__ float exponentials(float (&v)[PER], float top) {
 }
 template <bool SIGMOID>
 __device__ __forceinline__ float score_of(float l, float top, float total) {
-    return SIGMOID ? sigmoid(l) : l == -INFINITY ? 0.0f : expf(l - top) / total;      // (a logit that is open has a total of 1 or more)
+    return SIGMOID ? sigmoid<false>(l) : l == -INFINITY ? 0.0f : expf(l - top) / total;      // (a logit that is open has a total of 1 or more)
 }
 
 // The picks' shares of the sum of their scores (lane k: the k-th pick, l = -inf in the others and for closed ones) come from scores relative to
@@ -265,7 +271,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
             // The picks' sums as they are, and the largest that one which is left out can be.  s of a key: an exp (off by some 2 + 1.2 |l|
             // units in the last place; s (1 - s) <= 1/4 and |l| s (1 - s) < 0.23 of that), a sum and a quotient: below 3e-7.  s + bias and the
             // 32-bit form of the exact sum are rounded once each.  Neighbours that are more than 1e-6 (1 + |s + bias|) apart are in order.
-            const float hi = l > -INFINITY ? clean(sigmoid(l) + __ldg(p.bias + mine)) : -INFINITY;
+            const float hi = l > -INFINITY ? clean(sigmoid<false>(l) + __ldg(p.bias + mine)) : -INFINITY;
             float lo = __shfl_down_sync(0xffffffffu, hi, 1);
             if (lane == p.K - 1) lo = (next_key | kIndex) > kClosedKey ? key_value(next_key | kIndex) : -INFINITY;
             const bool unsettled = lane < p.K && lo > -INFINITY && !(hi - lo > 1e-6f + 1e-6f * fmaxf(fabsf(hi), fabsf(lo)));
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
         if (with_scores) {          // v: what d_score_sums is multiplied by, the scores or the sigmoid's slope
             if (SIGMOID) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) v[i] = sigmoid_slope(v[i]);
+                for (int i = 0; i < PER; ++i) v[i] = sigmoid_slope<true>(v[i]);
             } else {
                 top = v[0];
 #pragma unroll
@@ -440,9 +446,9 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
             }
             const float inv = norm > 0.0f ? 1.0f / norm : 0.0f;          // (norm is 1/2 or more where a pick is open)
             part = r * inv * (dw - mean * inv);
-            if (SIGMOID) part *= sigmoid(-l);          // 1 - s
+            if (SIGMOID) part *= sigmoid<false>(-l);          // 1 - s
         } else {
-            part = (SIGMOID ? sigmoid_slope(l) : score_of<false>(l, top, total)) * dw;
+            part = (SIGMOID ? sigmoid_slope<false>(l) : score_of<false>(l, top, total)) * dw;
             if (!SIGMOID) dot = part;                // (added up below, with the scores' own)
         }
         if (mine >= 0) tag_sm[mine] = static_cast<uint8_t>(lane);
