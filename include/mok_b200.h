@@ -542,8 +542,8 @@ int mokb_few_tokens_fwd(const mokb_few_tokens_args* args, void* stream);
  * Load figures (optional, together; scratch: mokb_route_scratch_bytes()): tokens_per_expert [num_experts] int32, picks of open
  * experts; score_sums [num_experts], the sum of s over the tokens in a fixed order.
  * mokb_route_bwd: d_logits [num_tokens, num_experts] without gaps, in the logits' type, from d_router_weights and (optional)
- * d_score_sums; top_experts are the forward call's (an entry outside [0, num_experts) is left out).  The picks themselves and
- * tokens_per_expert have no gradient. */
+ * d_score_sums; top_experts are the forward call's (an entry outside [0, num_experts), and one whose expert is closed, is left out,
+ * whatever d_router_weights holds there).  The picks themselves and tokens_per_expert have no gradient. */
 #define MOKB_SCORE_SOFTMAX 0
 #define MOKB_SCORE_SIGMOID 1
 #define MOKB_ROUTE_MAX_EXPERTS 1024

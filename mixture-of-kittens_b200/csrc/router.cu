@@ -416,8 +416,8 @@ __global__ void __launch_bounds__(route_threads(PER), route_blocks_per_sm(PER)) 
 #pragma unroll
         for (int i = 0; i < PER; ++i) v[i] = clean(next[i]);
         const int mine = next_pick >= 0 && next_pick < p.E ? static_cast<int>(next_pick) : -1;      // anything else has no logit
-        const float dw = mine >= 0 ? next_dw * p.scale : 0.0f;
         const float l = mine >= 0 ? load_clean<BF16>(p, row, mine) : -INFINITY;
+        const float dw = l > -INFINITY ? next_dw * p.scale : 0.0f;          // (a closed pick's weight is 0 for good)
         if (row + step < p.T) fetch(row + step);
         float top = 0.0f, total = 1.0f, dot = 0.0f;
         if (with_scores) {          // v: what d_score_sums is multiplied by, the scores or the sigmoid's slope

@@ -173,3 +173,24 @@ def test_long_batches_of_near_ties():
     bias = torch.randint(0, 3, (E,), generator=gen, device="cuda").float() * 2.0 ** -24
     r = F.route(F.MoKRouterConfig(topk=K, score="sigmoid"), logits, bias)
     assert torch.equal(r.top_experts, P.route(logits, K, "sigmoid", bias)[0])
+
+
+@pytest.mark.parametrize("with_sums", [False, True], ids=["weights", "sums"])
+@pytest.mark.parametrize("score,renorm", list(itertools.product(["softmax", "sigmoid"], [True, False])))
+def test_a_closed_pick_takes_no_gradient(score, renorm, with_sums):
+    """The weight of a closed expert is 0 whatever its logit: a NaN or an infinity in its place among d_router_weights is not looked at."""
+    from mok import functional as F
+    T, E, K = 64, 40, 6
+    logits = logits_of(T, E, torch.float32, seed=11, masked=0.9)
+    logits[5] = -torch.inf
+    cfg = F.MoKRouterConfig(topk=K, score=score, renormalize=renorm)
+    r = F.route(cfg, logits)
+    closed = torch.isneginf(logits.gather(1, r.top_experts))
+    assert closed.any() and not closed.all()
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    dw = torch.randn(T, K, generator=gen, device="cuda").masked_fill(closed, 0.0)
+    ds = torch.randn(E, generator=gen, device="cuda") if with_sums else None
+    want = F.route_backward(cfg, logits, r, dw, ds)
+    assert torch.isfinite(want).all()
+    for bad in (torch.nan, torch.inf, 1e30):
+        assert torch.equal(F.route_backward(cfg, logits, r, dw.masked_fill(closed, bad), ds), want)
